@@ -9,6 +9,8 @@ Public surface (same names as the reference):
     CachedPQMF                               diffusion/pqmf.py:236-302 (design + forward/inverse on libadk)
     AudioDenoiserModel, Denoiser             decoders/diffusion_decoder.py:261-337 (k-diffusion denoiser family)
     get_sigmas_karras, get_sigmas_exponential, sample_heun, sample_lms     diffusion/inference.py:60-73, 94-154
+    qk_norm_rope, rope_frequencies, masked_attention, alibi_slopes     attention operators of transformer denoisers over
+                                             token sequences, with gradients (transformer.py)
 Compute runs exclusively in libadk.so (hand-written gfx950 HIP kernels, C ABI in include/adk.h).
 """
 from .unet import DiffusionAttnUnet1D
@@ -17,7 +19,9 @@ from .sampling import (sample, sample_crash, sample_diffae, audio_to_int16, get_
                        sample_lms, to_d)
 from .pqmf import CachedPQMF
 from .kdiffusion import AudioDenoiserModel, Denoiser
+from .transformer import alibi_slopes, masked_attention, qk_norm_rope, rope_frequencies
 from . import _lib, blocks, distributed
 
 __all__ = ["DiffusionAttnUnet1D", "sample", "sample_crash", "sample_diffae", "audio_to_int16", "get_alphas_sigmas",
-           "alpha_sigma_to_t", "get_crash_schedule", "step_coefficients", "CachedPQMF", "AudioDenoiserModel", "Denoiser", "get_sigmas_karras", "get_sigmas_exponential", "sample_heun", "sample_lms", "to_d"]
+           "alpha_sigma_to_t", "get_crash_schedule", "step_coefficients", "CachedPQMF", "AudioDenoiserModel", "Denoiser", "get_sigmas_karras", "get_sigmas_exponential", "sample_heun", "sample_lms", "to_d",
+           "qk_norm_rope", "rope_frequencies", "masked_attention", "alibi_slopes"]

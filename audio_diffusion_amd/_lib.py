@@ -55,6 +55,40 @@ class AdkOp(C.Structure):
     ]
 
 
+def _fields(text):
+    """ctypes fields from 'type name name ...' lines: the structs below are written as include/adk.h has them."""
+    types = {"i32": C.c_int32, "i64": C.c_int64, "f32": C.c_float, "ptr": C.c_void_p}
+    return [(name, types[line.split()[0]]) for line in text.strip().splitlines() for name in line.split()[1:]]
+
+
+class QkNormRopeArgs(C.Structure):
+    """Mirror of ``adk_qk_norm_rope_args`` (include/adk.h)."""
+    _fields_ = _fields("""
+        i32 dtype B N Hq Hk D R interleaved pos_bytes
+        f32 eps
+        ptr q k
+        i64 q_stride_b q_stride_n q_stride_h k_stride_b k_stride_n k_stride_h
+        ptr q_weight k_weight positions
+        i64 pos_stride_b pos_stride_n
+        ptr frequencies q_out k_out q_grad k_grad
+        i64 qg_stride_b qg_stride_n qg_stride_h kg_stride_b kg_stride_n kg_stride_h
+        ptr q_weight_grad k_weight_grad""")
+
+
+class AttentionArgs(C.Structure):
+    """Mirror of ``adk_attention_args`` (include/adk.h)."""
+    _fields_ = _fields("""
+        i32 dtype B Nq Nk Hq Hk D causal
+        f32 scale softcap
+        ptr q k v
+        i64 q_stride_b q_stride_n q_stride_h k_stride_b k_stride_n k_stride_h v_stride_b v_stride_n v_stride_h
+        ptr slopes prefix lengths starts documents
+        i64 documents_stride
+        ptr o lse o_grad
+        i64 og_stride_b og_stride_n og_stride_h
+        ptr q_grad k_grad v_grad""")
+
+
 EXPORTS = [
     "adk_version", "adk_last_error", "adk_sizeof_op", "adk_run_plan", "adk_validate_plan", "adk_partials_count", "adk_conv_postile", "adk_conv_cotile_used", "adk_conv_cotile",
     "adk_conv1d", "adk_gn_apply", "adk_gn_stats", "adk_fir_down2", "adk_fir_up2", "adk_attn1d",
@@ -62,6 +96,8 @@ EXPORTS = [
     "adk_ddim_update", "adk_step_advance", "adk_audio_to_int16", "adk_space_to_depth", "adk_depth_to_space",
     "adk_attn1d_hd", "adk_adagn_apply", "adk_linear", "adk_fourier_features", "adk_pack_input_plain",
     "adk_unpack_output_scaled", "adk_group_norm_noalloc", "adk_conv_gn_fusable",
+    "adk_sizeof_qk_norm_rope", "adk_qk_norm_rope", "adk_qk_norm_rope_workspace", "adk_qk_norm_rope_backward",
+    "adk_sizeof_attention", "adk_attention", "adk_attention_workspace", "adk_attention_backward",
 ]
 
 _lib = None
@@ -116,9 +152,18 @@ def load():
     lib.adk_pack_input_plain.argtypes = [i32, i32, i32, i32, i32, vp, vp, vp, i32, i32, vp, vp]
     lib.adk_unpack_output_scaled.argtypes = [i32, i32, i32, i32, vp, vp, vp, vp, vp, vp]
     lib.adk_group_norm_noalloc.argtypes = [i32, u32, i32, i32, i32, i32, f32, vp, vp, vp, vp, vp, vp]
+    lib.adk_qk_norm_rope.argtypes = [C.POINTER(QkNormRopeArgs), vp]
+    lib.adk_qk_norm_rope_workspace.argtypes = [C.POINTER(QkNormRopeArgs)]
+    lib.adk_qk_norm_rope_backward.argtypes = [C.POINTER(QkNormRopeArgs), vp, i64, vp]
+    lib.adk_attention.argtypes = [C.POINTER(AttentionArgs), vp, i64, vp]
+    lib.adk_attention_workspace.argtypes = [C.POINTER(AttentionArgs), i32]
+    lib.adk_attention_backward.argtypes = [C.POINTER(AttentionArgs), vp, i64, vp]
     for name in EXPORTS:
         if name not in ("adk_last_error",):
-            getattr(lib, name).restype = C.c_int
+            getattr(lib, name).restype = i64 if name.endswith("_workspace") else C.c_int
+    for name, mirror in (("adk_sizeof_qk_norm_rope", QkNormRopeArgs), ("adk_sizeof_attention", AttentionArgs)):
+        if getattr(lib, name)() != C.sizeof(mirror):
+            raise AdkError(f"libadk.so was built from another include/adk.h ({name}() != {C.sizeof(mirror)})")
     _lib = lib
     return lib
 

@@ -4,7 +4,7 @@
 #include <stdio.h>
 #include <string.h>
 #include <mutex>
-#include "adk_common.h"
+#include "masked_attention.h"
 
 int launch_conv(const adk_op& op, hipStream_t st);
 int conv_cotile(int Cout);
@@ -26,6 +26,10 @@ int launch_audio_to_int16(const adk_op& op, hipStream_t st);
 int launch_phase_shuffle(const adk_op& op, hipStream_t st, bool to_depth);
 int launch_linear(const adk_op& op, hipStream_t st);
 int launch_fourier(const adk_op& op, hipStream_t st);
+int launch_qk_norm_rope(const adk_qk_norm_rope_args& a, void* ws, hipStream_t st, bool grad);
+long long qk_norm_rope_workspace(const adk_qk_norm_rope_args& a);
+long long att_forward_workspace(const AttArgs& a);
+long long att_backward_workspace(const AttArgs& a);
 
 static thread_local char g_err[512] = "";
 
@@ -543,6 +547,111 @@ int adk_group_norm_noalloc(int dtype, uint32_t flags, int B, int L, int P, int C
     if ((rc = dispatch(s, st)) || (rc = dispatch(o, st)))
         return fail(rc, "group_norm_noalloc: launch failed: %s", hipGetErrorString(hipGetLastError()));
     return ADK_OK;
+}
+
+
+// ---- operators on token sequences ------------------------------------------------------------------------------------------
+static int check_qk(const adk_qk_norm_rope_args* a, bool grad, const char* what)
+{
+    REQUIRE(a, "%s: null arguments", what);
+    REQUIRE(a->dtype == ADK_F32 || a->dtype == ADK_BF16 || a->dtype == ADK_F16, "%s: dtype %d unsupported", what, a->dtype);
+    REQUIRE(a->B >= 0 && a->N >= 0 && (long long)a->B * a->N < (1LL << 31), "%s: B=%d N=%d (fewer than 2^31 rows)", what, a->B, a->N);
+    REQUIRE(a->Hq >= 1 && a->Hk >= 1 && a->Hq <= 65536 && a->Hk <= 65536, "%s: heads Hq=%d Hk=%d outside [1, 65536]", what, a->Hq, a->Hk);
+    REQUIRE(a->D >= 2 && a->D <= 256 && a->D % 2 == 0, "%s: head dim %d is not even in [2, 256]", what, a->D);
+    REQUIRE(a->R >= 0 && a->R <= a->D && a->R % 2 == 0, "%s: rotated elements R=%d are not even in [0, D=%d]", what, a->R, a->D);
+    REQUIRE(a->eps > 0.f, "%s: eps=%g", what, (double)a->eps);
+    REQUIRE(a->pos_bytes == 4 || a->pos_bytes == 8, "%s: positions of %d bytes (4 or 8)", what, a->pos_bytes);
+    if (a->B == 0 || a->N == 0) return ADK_OK;             // nothing is read
+    REQUIRE(a->q && a->k && a->q_out && a->k_out && a->positions && (a->frequencies || a->R == 0), "%s: null tensor", what);
+    REQUIRE(!grad || (a->q_grad && a->k_grad), "%s: null gradient", what);
+    const uintptr_t el = a->dtype == ADK_F32 ? 3 : 1;
+    REQUIRE(!(((uintptr_t)a->q | (uintptr_t)a->k | (uintptr_t)a->q_out | (uintptr_t)a->k_out) & el)
+            && !(grad && (((uintptr_t)a->q_grad | (uintptr_t)a->k_grad) & el)), "%s: a tensor is not aligned to its elements", what);
+    return ADK_OK;
+}
+
+int adk_sizeof_qk_norm_rope(void) { return (int)sizeof(adk_qk_norm_rope_args); }
+int adk_sizeof_attention(void) { return (int)sizeof(adk_attention_args); }
+
+int adk_qk_norm_rope(const adk_qk_norm_rope_args* a, void* stream)
+{
+    const int rc = check_qk(a, false, "qk_norm_rope");
+    if (rc || a->B == 0 || a->N == 0) return rc;
+    const int lr = launch_qk_norm_rope(*a, nullptr, reinterpret_cast<hipStream_t>(stream), false);
+    return lr ? fail(lr, "qk_norm_rope: launch failed: %s", hipGetErrorString(hipGetLastError())) : ADK_OK;
+}
+
+int64_t adk_qk_norm_rope_workspace(const adk_qk_norm_rope_args* a)
+{
+    if (check_qk(a, false, "qk_norm_rope")) return -1;
+    return qk_norm_rope_workspace(*a);
+}
+
+int adk_qk_norm_rope_backward(const adk_qk_norm_rope_args* a, void* ws, int64_t ws_bytes, void* stream)
+{
+    int rc = check_qk(a, true, "qk_norm_rope_backward");
+    if (rc) return rc;
+    REQUIRE((a->B > 0 && a->N > 0) || (!a->q_weight_grad && !a->k_weight_grad), "qk_norm_rope_backward: no rows to sum a weight gradient over");
+    if (a->B == 0 || a->N == 0) return ADK_OK;
+    REQUIRE(ws && ((uintptr_t)ws & 15) == 0 && ws_bytes >= qk_norm_rope_workspace(*a), "qk_norm_rope_backward: workspace of %lld bytes, needs %lld",
+            (long long)ws_bytes, qk_norm_rope_workspace(*a));
+    rc = launch_qk_norm_rope(*a, ws, reinterpret_cast<hipStream_t>(stream), true);
+    return rc ? fail(rc, "qk_norm_rope_backward: launch failed: %s", hipGetErrorString(hipGetLastError())) : ADK_OK;
+}
+
+static int check_att(const AttArgs* a, bool grad, const char* what)
+{
+    REQUIRE(a, "%s: null arguments", what);
+    REQUIRE(a->dtype == ADK_BF16 || a->dtype == ADK_F16, "%s: dtype %d unsupported (bf16 or f16)", what, a->dtype);
+    REQUIRE(a->D == 32 || a->D == 64 || a->D == 128, "%s: head dim %d unsupported (32, 64 or 128)", what, a->D);
+    REQUIRE(a->Hq >= 1 && a->Hk >= 1 && a->Hq % a->Hk == 0, "%s: %d query heads are not a multiple of %d key heads", what, a->Hq, a->Hk);
+    REQUIRE(a->B >= 0 && a->Nq >= 0 && a->Nk >= 0 && a->Nq <= (1 << 28) && a->Nk <= (1 << 28), "%s: B=%d Nq=%d Nk=%d (lengths up to 2^28)",
+            what, a->B, a->Nq, a->Nk);
+    REQUIRE(a->B <= 65535 && (long long)a->B * a->Hq * ((a->Nq + 31LL) / 32) < (1LL << 30) && (long long)a->B * a->Hk * ((a->Nk + 31LL) / 32) < (1LL << 30)
+            && (long long)a->Nq * (a->Hq / a->Hk) < (1LL << 30), "%s: B=%d x heads %d / %d x rows %d / %d exceed the grid", what, a->B, a->Hq, a->Hk, a->Nq, a->Nk);
+    REQUIRE(a->scale > 0.f && a->scale <= 3.0e38f, "%s: scale=%g must be positive and finite", what, (double)a->scale);
+    REQUIRE(a->softcap >= 0.f && a->softcap <= 3.0e38f, "%s: softcap=%g must be positive and finite, or 0", what, (double)a->softcap);
+    REQUIRE(a->causal || !a->prefix, "%s: a prefix mask widens a causal one: set causal", what);
+    if (a->B == 0 || a->Nq == 0) return ADK_OK;            // no rows
+    REQUIRE(a->q && a->o && (a->Nk == 0 || (a->k && a->v)), "%s: null tensor", what);
+    auto al = [](const void* p) { return ((uintptr_t)p & 15) == 0; };
+    auto s8 = [](int64_t x, int64_t y, int64_t z) { return x % 8 == 0 && y % 8 == 0 && z % 8 == 0; };
+    REQUIRE(al(a->q) && al(a->k) && al(a->v) && al(a->o), "%s: q, k, v and o must be 16-byte aligned", what);
+    REQUIRE(s8(a->q_stride_b, a->q_stride_n, a->q_stride_h) && s8(a->k_stride_b, a->k_stride_n, a->k_stride_h)
+            && s8(a->v_stride_b, a->v_stride_n, a->v_stride_h), "%s: strides must be multiples of 8 elements", what);
+    if (grad) {
+        REQUIRE(a->lse && a->o_grad && a->q_grad && (a->Nk == 0 || (a->k_grad && a->v_grad)), "%s: null tensor", what);
+        REQUIRE(al(a->o_grad) && al(a->q_grad) && al(a->k_grad) && al(a->v_grad) && s8(a->og_stride_b, a->og_stride_n, a->og_stride_h),
+                "%s: gradients must be 16-byte aligned with strides of multiples of 8 elements", what);
+    }
+    return ADK_OK;
+}
+
+int64_t adk_attention_workspace(const adk_attention_args* a, int backward)
+{
+    if (check_att(a, false, "attention")) return -1;
+    return backward ? att_backward_workspace(*a) : att_forward_workspace(*a);
+}
+
+static int run_att(const AttArgs* a, void* ws, int64_t ws_bytes, void* stream, bool grad, const char* what)
+{
+    const int rc = check_att(a, grad, what);
+    if (rc) return rc;
+    REQUIRE(!grad || a->B == 0 || a->Nq > 0, "%s: no query rows (the gradients of k and v are zeros)", what);
+    if (a->B == 0 || a->Nq == 0) return ADK_OK;
+    const long long need = grad ? att_backward_workspace(*a) : att_forward_workspace(*a);
+    REQUIRE(need == 0 || (ws && ((uintptr_t)ws & 15) == 0 && ws_bytes >= need), "%s: workspace of %lld bytes, needs %lld", what,
+            (long long)ws_bytes, need);
+    hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+    const int lr = grad ? (a->dtype == ADK_BF16 ? att_backward_bf16(*a, ws, st) : att_backward_f16(*a, ws, st))
+                        : (a->dtype == ADK_BF16 ? att_forward_bf16(*a, ws, st) : att_forward_f16(*a, ws, st));
+    return lr ? fail(lr, "%s: launch failed: %s", what, hipGetErrorString(hipGetLastError())) : ADK_OK;
+}
+
+int adk_attention(const adk_attention_args* a, void* ws, int64_t ws_bytes, void* stream) { return run_att(a, ws, ws_bytes, stream, false, "attention"); }
+int adk_attention_backward(const adk_attention_args* a, void* ws, int64_t ws_bytes, void* stream)
+{
+    return run_att(a, ws, ws_bytes, stream, true, "attention_backward");
 }
 
 }  // extern "C"

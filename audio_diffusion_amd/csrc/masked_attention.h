@@ -1,0 +1,236 @@
+// Shared parts of the masked attention kernels (masked_attention_fwd.inc, _step.inc, _bwd.inc): the mask of a query row as a key
+// limit and a document, the score transform, LDS tiles of keys (or query rows) and their fragments.
+//
+// All kernels keep ONE index of a score tile on the lane: a 32 x 32 tile of S^T = K Q^T (or S = Q K^T) comes out of
+// v_mfma_f32_32x32x16 with column = lane & 31 and rows (r & 3) + 8 (r >> 2) + 4 (lane >> 5), r = 0..15, and those 16 registers,
+// rounded to 16 bits, are the B operand of the next product as they stand: neither scores nor probabilities touch LDS.
+#pragma once
+#include "adk_common.h"
+
+typedef adk_attention_args AttArgs;
+typedef __attribute__((ext_vector_type(4))) short att_s16x4;
+
+constexpr int AT_KT = 64;                    // keys of one LDS tile, and of one entry of the document ranges
+constexpr float AT_LOG2E = 1.44269504088896340736f;
+
+template <typename T> struct SeqMma;
+template <> struct SeqMma<bf16_t> {
+    typedef bf16x8 Frag;
+    static __device__ __forceinline__ f32x16 run(const Frag& a, const Frag& b, const f32x16& c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+};
+template <> struct SeqMma<f16_t> {
+    typedef f16x8 Frag;
+    static __device__ __forceinline__ f32x16 run(const Frag& a, const Frag& b, const f32x16& c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+};
+
+__device__ __forceinline__ f32x16 at_zero16()
+{
+    f32x16 z;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) z[r] = 0.f;
+    return z;
+}
+// row of register r of a 32 x 32 tile, less the lane half's 4 h
+__device__ __forceinline__ constexpr int at_row(int r) { return (r & 3) + 8 * (r >> 2); }
+
+__device__ __forceinline__ float at_xhalf_max(float x)
+{
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float at_xhalf_sum(float x)
+{
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// ---- masks ---------------------------------------------------------------------------------------------------------------
+// Causal, prefix and length masks together are one limit per row: key j is seen if j <= lim.  lim grows with the row, so
+// the first and last row of a tile bound it.  Documents are an equality on top; a row without one gets the limit -1.
+struct AtSample { int klen, start, prefix; };
+
+__device__ __forceinline__ AtSample at_sample(const AttArgs& a, int b)
+{
+    AtSample s;
+    s.klen = a.lengths ? min(max(a.lengths[b], 0), a.Nk) : a.Nk;
+    s.start = a.starts ? min(max(a.starts[b], -(1 << 29)), 1 << 29) : a.Nk - a.Nq;
+    s.prefix = a.prefix ? a.prefix[b] : 0;
+    return s;
+}
+__device__ __forceinline__ int at_limit(const AttArgs& a, const AtSample& s, int i)
+{
+    return a.causal ? min(s.klen - 1, max(s.start + i, s.prefix - 1)) : s.klen - 1;
+}
+// The position a distance is taken from: outside the keys the distances differ from those of the nearest end by a constant
+// of the row, which the softmax does not see.
+__device__ __forceinline__ float at_bias_pos(const AttArgs& a, const AtSample& s, int i) { return (float)min(max(s.start + i, 0), a.Nk - 1); }
+__device__ __forceinline__ int at_row_doc(const AttArgs& a, const AtSample& s, int b, int i)       // negative: none
+{
+    const int p = s.start + i;
+    if (p < 0 || p >= a.Nk) return -1;
+    return a.documents[(long long)b * a.documents_stride + p];
+}
+// smallest and largest document of the rows that have one (empty: lo > hi), over all 64 lanes; and whether all 64 have it
+struct AtDocs { int lo, hi; bool one; };
+__device__ __forceinline__ AtDocs at_doc_range(int doc)
+{
+    AtDocs d;
+    d.lo = doc < 0 ? 0x7fffffff : doc;
+    d.hi = doc < 0 ? -1 : doc;
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) {
+        d.lo = min(d.lo, __shfl_xor(d.lo, m, 64));
+        d.hi = max(d.hi, __shfl_xor(d.hi, m, 64));
+    }
+    d.lo = __builtin_amdgcn_readfirstlane(d.lo);
+    d.hi = __builtin_amdgcn_readfirstlane(d.hi);
+    d.one = __ballot(doc != d.lo) == 0ull;
+    return d;
+}
+// [lo, hi] of documents; entry t of the ranges of the 64-key tiles by a scalar load (t is wave-uniform)
+struct AtRange { int lo, hi; };
+__device__ __forceinline__ AtRange at_range(const int* ranges, int t)
+{
+    const auto* p = (const __attribute__((address_space(4))) int*)(ranges + 2 * (long long)t);
+    return {p[0], p[1]};
+}
+__device__ __forceinline__ bool at_meet(const AtRange& r, int lo, int hi) { return r.lo <= hi && r.hi >= lo; }
+
+// ---- scores --------------------------------------------------------------------------------------------------------------
+// base-2 scores: x = score * log2(e).  Plain: x = qk * c.  Capped: c tanh(t) = c (1 - 2 / (exp(2 t) + 1)), t = qk * scale / cap.
+struct AtScore { float c, k1, capl2; };      // scale * log2 e;  2 log2 e scale / cap;  cap * log2 e
+
+static inline AtScore at_score_of(const AttArgs& a)
+{
+    AtScore s;
+    s.c = a.scale * AT_LOG2E;
+    s.k1 = a.softcap > 0.f ? 2.f * AT_LOG2E * a.scale / a.softcap : 0.f;
+    s.capl2 = a.softcap * AT_LOG2E;
+    return s;
+}
+__device__ __forceinline__ float at_tanh(float qk, float k1)
+{
+    return 1.f - 2.f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(qk * k1) + 1.f);
+}
+
+// ---- LDS tiles -----------------------------------------------------------------------------------------------------------
+// A tile is [rows][D] 16-bit, rows of 2 D bytes, filled by LDS-DMA (1 KiB per wave instruction, lane l at + 16 l).  Piece p
+// (16 bytes) of row r sits in slot p ^ swz(r): reading one piece of 8 consecutive rows (row fragments) and 4 pieces of
+// 4 consecutive rows (transposed fragments) then both cover the banks evenly.
+template <int D> __device__ __forceinline__ int at_swz(int row)
+{
+    constexpr int hi_shift = D == 128 ? 0 : D == 64 ? 1 : 2;
+    const int hi = (row >> hi_shift) & (D / 32 - 1), lo = (row >> 2) & 3;
+    return (hi << 2) | lo;
+}
+__device__ __forceinline__ void at_dma16(const void* src, unsigned char* lds)
+{
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
+                                     (__attribute__((address_space(3))) void*)lds, 16, 0, 0);
+}
+// 64 ints, one per lane, to lds + 4 lane
+__device__ __forceinline__ void at_dma4(const void* src, unsigned char* lds)
+{
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
+                                     (__attribute__((address_space(3))) void*)lds, 4, 0, 0);
+}
+// ROWS x D rows starting at `row0` (rows past `last` repeat it) of a tensor with row stride `stride` elements; wave `wave`
+// of NW takes its share.  base points at row 0.
+template <int D, int ROWS, int NW>
+__device__ __forceinline__ void at_load_tile(const unsigned char* base, long long stride, int row0, int last, unsigned char* lds, int wave, int lane)
+{
+    constexpr int PPR = D / 8, RPI = 64 / PPR, NI = ROWS / RPI;          // pieces per row, rows per instruction
+    static_assert(NI % NW == 0, "every wave issues the same number of loads");
+#pragma unroll
+    for (int t = 0; t < NI / NW; ++t) {
+        const int instr = wave * (NI / NW) + t;
+        const int row = instr * RPI + lane / PPR;
+        const int piece = (lane % PPR) ^ at_swz<D>(row);
+        const int gr = min(row0 + row, last);
+        at_dma16(base + ((long long)gr * stride + piece * 8) * 2, lds + instr * 1024);
+    }
+}
+// Row fragment (A or B operand, contraction over d): lane (row = lane & 31, h) gets elements 16 ks + 8 h .. + 7 of row
+// row0 + (lane & 31).  `addr` = at_row_addr(lane), kept by the caller.
+template <int D> __device__ __forceinline__ int at_row_addr(int lane) { const int r = lane & 31; return r * 2 * D + (((lane >> 5) ^ at_swz<D>(r)) << 4); }
+template <int D, typename Frag> __device__ __forceinline__ Frag at_row_frag(const unsigned char* tile, int addr, int row0, int ks)
+{
+    return *reinterpret_cast<const Frag*>(tile + row0 * 2 * D + (addr ^ (ks << 5)));     // row0 a multiple of 32
+}
+// Transposed fragment (A operand X^T, contraction over the tile's rows): lane (d = 32 dt + (lane & 31), h) gets rows
+// row0 + 16 s + {4 h + 0..3, 8 + 4 h + 0..3}: the order in which the score registers 8 s .. 8 s + 7 hold them.
+template <int D> __device__ __forceinline__ int at_tr_addr(int lane, int u)
+{
+    const int r = 8 * u + 4 * (lane >> 5) + ((lane & 15) >> 2);
+    const int piece = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+    return r * 2 * D + ((piece ^ at_swz<D>(r)) << 4) + (lane & 1) * 8;
+}
+template <int D, typename Frag> __device__ __forceinline__ Frag at_tr_frag(const unsigned char* tile, const int (&addr)[2], int row0, int s, int dt)
+{
+    union { att_s16x4 v[2]; Frag f; } cv;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+        cv.v[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (__attribute__((address_space(3))) att_s16x4*)(tile + (row0 + 16 * s) * 2 * D + (addr[u] ^ (dt << 6))));
+    return cv.f;
+}
+
+// 16 f32 -> two B operands (registers 0..7, 8..15)
+template <typename T> __device__ __forceinline__ void at_pack(const f32x16& p, typename SeqMma<T>::Frag (&f)[2])
+{
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+        union { uint32_t w[4]; typename SeqMma<T>::Frag f; } cv;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) cv.w[e] = pack2v(f32x2{p[8 * s + 2 * e], p[8 * s + 2 * e + 1]}, T());
+        f[s] = cv.f;
+    }
+}
+
+// ---- the key tiles that a block of query rows walks (forward and dQ) -----------------------------------------------------------
+// First and last tile that any row of the block sees, found by all threads over the ranges of documents; tiles between them
+// that miss the block's documents are stepped over.
+template <int NW> struct AtWalk {
+    const int* ranges;          // of the sample, or nullptr: no documents
+    int t0, t1, lo, hi;
+    __device__ __forceinline__ int next(int t) const
+    {
+        ++t;
+        if (ranges) while (t < t1 && !at_meet(at_range(ranges, t), lo, hi)) ++t;
+        return t;
+    }
+};
+template <int NW>
+__device__ __forceinline__ AtWalk<NW> at_walk(const AttArgs& a, const int* all_ranges, int b, int last_limit, int lo, int hi, int* red)
+{
+    AtWalk<NW> w;
+    const int tid = threadIdx.x;
+    w.ranges = nullptr; w.t0 = 0; w.lo = lo; w.hi = hi;
+    w.t1 = last_limit < 0 ? 0 : last_limit / AT_KT + 1;
+    if (a.documents && w.t1) {
+        w.ranges = all_ranges + (long long)b * ((a.Nk + AT_KT - 1) / AT_KT) * 2;
+        if ((tid & 63) == 0) { red[2 * (tid >> 6)] = lo; red[2 * (tid >> 6) + 1] = hi; }
+        if (tid == 0) { red[2 * NW] = 0x7fffffff; red[2 * NW + 1] = 0; }
+        __syncthreads();
+        for (int v = 0; v < NW; ++v) { lo = min(lo, red[2 * v]); hi = max(hi, red[2 * v + 1]); }
+        int first = 0x7fffffff, end = 0;
+        for (int t = tid; t < w.t1; t += 64 * NW)
+            if (w.ranges[2 * (long long)t] <= hi && w.ranges[2 * (long long)t + 1] >= lo) { first = min(first, t); end = t + 1; }
+        if (end) { atomicMin(&red[2 * NW], first); atomicMax(&red[2 * NW + 1], end); }       // min and max: any order, one result
+        __syncthreads();
+        w.t0 = __builtin_amdgcn_readfirstlane(red[2 * NW]);
+        w.t1 = __builtin_amdgcn_readfirstlane(red[2 * NW + 1]);
+        w.lo = __builtin_amdgcn_readfirstlane(lo); w.hi = __builtin_amdgcn_readfirstlane(hi);
+    }
+    return w;
+}
+
+// ---- launchers (one translation unit per type) -----------------------------------------------------------------------------
+int att_forward_bf16(const AttArgs& a, void* ws, hipStream_t st);
+int att_forward_f16(const AttArgs& a, void* ws, hipStream_t st);
+int att_backward_bf16(const AttArgs& a, void* ws, hipStream_t st);
+int att_backward_f16(const AttArgs& a, void* ws, hipStream_t st);
+int att_launch_doc_ranges(const AttArgs& a, int* ranges, hipStream_t st);
+static inline int att_key_tiles(const AttArgs& a) { return (a.Nk + AT_KT - 1) / AT_KT; }
+constexpr int AT_DOC_LDS = AT_KT * 4;        // documents of a tile, behind its rows
+static inline long long att_doc_bytes(const AttArgs& a) { return a.documents ? (((long long)a.B * att_key_tiles(a) * 8 + 255) & ~255LL) : 0; }

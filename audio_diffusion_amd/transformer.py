@@ -1,0 +1,288 @@
+"""Operators of transformer denoisers over token (latent) sequences, on libadk: per-head RMS norm of queries and keys with
+the position rotation, and softmax attention with capped scores, a distance bias and causal / prefix / document / length masks.
+
+They take rows ``[B, N, heads, head_dim]`` as a linear projection leaves them (views of one packed projection included) and
+carry gradients.  Every call runs on the current stream of its tensors' device; outputs and workspaces come from torch's
+allocator on that stream, so a call can be captured in a graph.  No CPU or eager fallback.
+"""
+import ctypes as C
+import math
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+
+__all__ = ["qk_norm_rope", "rope_frequencies", "masked_attention", "alibi_slopes"]
+
+_NORM_TYPES = {torch.float32: _lib.ADK_F32, torch.bfloat16: _lib.ADK_BF16, torch.float16: _lib.ADK_F16}
+_ATT_TYPES = {torch.bfloat16: _lib.ADK_BF16, torch.float16: _lib.ADK_F16}
+
+
+def rope_frequencies(rotary_dim, base=10000.0, device=None):
+    """float64 ``[rotary_dim / 2]`` radians per position: base ** (-2 p / rotary_dim)."""
+    if rotary_dim < 0 or rotary_dim % 2:
+        raise ValueError(f"rotary_dim {rotary_dim} is not even")
+    p = torch.arange(rotary_dim // 2, dtype=torch.float64, device=device)
+    return float(base) ** (-2.0 * p / max(rotary_dim, 1))
+
+
+def alibi_slopes(heads, device=None):
+    """float32 ``[heads]`` distance-bias slopes, the geometric series 2 ** (-8 (h + 1) / heads)."""
+    return torch.exp2(-8.0 * torch.arange(1, heads + 1, dtype=torch.float64, device=device) / heads).float()
+
+
+def _need(ok, message, kind=ValueError):
+    if not ok:
+        raise kind(message)
+
+
+def _on_device(what, device, *tensors):
+    _need(device.type == "cuda", f"{what}: tensors are on {device}; there is no CPU path", RuntimeError)
+    for t in tensors:
+        _need(t is None or t.device == device, f"{what}: tensors on {t.device if t is not None else ''} and {device}")
+
+
+def _rows(t):
+    """Rows as the kernels read them: the elements of a head contiguous (a copy if they are not)."""
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _rows16(t):
+    """Rows with 16-byte aligned heads (a copy if they are not)."""
+    sb, sn, sh, sd = t.stride()
+    if sd == 1 and not ((sb | sn | sh) & 7) and not (t.data_ptr() & 15):
+        return t
+    t = t.contiguous()
+    return t if not (t.data_ptr() & 15) else t.clone()
+
+
+class _Device:
+    """Makes a device current for the launches of a call (a no-op where it is already)."""
+    __slots__ = ("want", "guard")
+
+    def __init__(self, device):
+        self.want, self.guard = device.index, None
+
+    def __enter__(self):
+        if torch.cuda.current_device() != self.want:
+            self.guard = torch.cuda.device(self.want)
+            self.guard.__enter__()
+        return C.c_void_p(torch.cuda.current_stream().cuda_stream)
+
+    def __exit__(self, *e):
+        if self.guard is not None:
+            self.guard.__exit__(*e)
+
+
+def _workspace(n, device):
+    """(tensor that owns it, pointer, bytes) of n bytes."""
+    if n <= 0:
+        return None, None, 0
+    w = torch.empty(n, dtype=torch.uint8, device=device)
+    return w, C.c_void_p(w.data_ptr()), n
+
+
+# ---- per-head norm and rotation -------------------------------------------------------------------------------------------
+
+def _norm_args(q, k, q_weight, k_weight, positions, frequencies, eps, interleaved):
+    B, N, Hq, D = q.shape
+    a = _lib.QkNormRopeArgs()
+    a.dtype, a.B, a.N, a.Hq, a.Hk, a.D, a.R = _NORM_TYPES[q.dtype], B, N, Hq, k.shape[2], D, 2 * frequencies.shape[0]
+    a.interleaved, a.eps = int(interleaved), eps
+    a.q, a.k = q.data_ptr(), k.data_ptr()
+    a.q_stride_b, a.q_stride_n, a.q_stride_h = q.stride()[:3]
+    a.k_stride_b, a.k_stride_n, a.k_stride_h = k.stride()[:3]
+    a.q_weight = q_weight.data_ptr() if q_weight is not None else None
+    a.k_weight = k_weight.data_ptr() if k_weight is not None else None
+    a.pos_bytes, a.positions = positions.element_size(), positions.data_ptr()
+    a.pos_stride_b, a.pos_stride_n = positions.stride()
+    a.frequencies = frequencies.data_ptr()
+    return a
+
+
+class _QkNormRope(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, q_weight, k_weight, positions, frequencies, eps, interleaved):
+        a = _norm_args(q, k, q_weight, k_weight, positions, frequencies, eps, interleaved)
+        qo, ko = torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(k.shape, dtype=k.dtype, device=q.device)
+        a.q_out, a.k_out = qo.data_ptr(), ko.data_ptr()
+        with _Device(q.device) as stream:
+            _lib.check(_lib.load().adk_qk_norm_rope(C.byref(a), stream), "qk_norm_rope")
+        ctx.save_for_backward(q, k, q_weight, k_weight, positions, frequencies)
+        ctx.eps, ctx.interleaved = eps, interleaved
+        return qo, ko
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gq, gk):
+        q, k, q_weight, k_weight, positions, frequencies = ctx.saved_tensors
+        a = _norm_args(q, k, q_weight, k_weight, positions, frequencies, ctx.eps, ctx.interleaved)
+        gq, gk = _rows(gq), _rows(gk)
+        dq, dk = torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(k.shape, dtype=k.dtype, device=q.device)
+        a.q_out, a.k_out, a.q_grad, a.k_grad = dq.data_ptr(), dk.data_ptr(), gq.data_ptr(), gk.data_ptr()
+        a.qg_stride_b, a.qg_stride_n, a.qg_stride_h = gq.stride()[:3]
+        a.kg_stride_b, a.kg_stride_n, a.kg_stride_h = gk.stride()[:3]
+        rows = q.shape[0] * q.shape[1]
+        make = torch.empty_like if rows else torch.zeros_like
+        dqw = make(q_weight) if q_weight is not None and ctx.needs_input_grad[2] else None
+        dkw = make(k_weight) if k_weight is not None and ctx.needs_input_grad[3] else None
+        if rows:
+            a.q_weight_grad = dqw.data_ptr() if dqw is not None else None
+            a.k_weight_grad = dkw.data_ptr() if dkw is not None else None
+            lib = _lib.load()
+            with _Device(q.device) as stream:
+                own, ws, n = _workspace(lib.adk_qk_norm_rope_workspace(C.byref(a)), q.device)
+                _lib.check(lib.adk_qk_norm_rope_backward(C.byref(a), ws, n, stream), "qk_norm_rope backward")
+        return dq, dk, dqw, dkw, None, None, None, None
+
+
+def qk_norm_rope(q, k, q_weight, k_weight, positions, frequencies, eps=1e-6, interleaved=False):
+    """RMS norm of every head of ``q`` [B, N, Hq, D] and ``k`` [B, N, Hk, D], times the weights, then the rotation of the
+    first ``2 * len(frequencies)`` elements by ``positions * frequencies``, in one pass; returns new contiguous (q, k).
+
+    * float32, bfloat16 or float16; D even up to 256; any strides (rows whose elements are not contiguous are copied first).
+    * ``q_weight`` / ``k_weight``: [D] of any floating type, or None for ones (computed and differentiated in float32).
+    * ``positions``: int32 or int64, [N] or [B, N], any values (expanded views are read as they are).
+    * ``frequencies``: float64 [R / 2], radians per position (``rope_frequencies``); may be empty (norm only).
+    * ``interleaved``: pairs (2p, 2p + 1) instead of (p, p + R / 2).
+    Gradients flow to q, k and the weights, not to positions or frequencies.
+    """
+    what = "qk_norm_rope"
+    _need(q.dim() == 4 and k.dim() == 4 and q.shape[:2] == k.shape[:2] and q.shape[3] == k.shape[3],
+          f"{what}: q {tuple(q.shape)} and k {tuple(k.shape)} are not [B, N, Hq, D] and [B, N, Hk, D]")
+    _need(q.dtype in _NORM_TYPES and k.dtype == q.dtype, f"{what}: q is {q.dtype}, k {k.dtype} (float32, bfloat16 or float16, both alike)")
+    B, N, _, D = q.shape
+    _need(D % 2 == 0 and 2 <= D <= 256, f"{what}: head dim {D} is not even in [2, 256]")
+    _need(q.shape[2] >= 1 and k.shape[2] >= 1, f"{what}: no heads")
+    _need(frequencies.dim() == 1 and frequencies.dtype == torch.float64, f"{what}: frequencies must be float64 [R / 2]")
+    _need(2 * frequencies.shape[0] <= D, f"{what}: {frequencies.shape[0]} frequencies turn more than the {D} elements of a head")
+    _need(positions.dtype in (torch.int32, torch.int64), f"{what}: positions are {positions.dtype} (int32 or int64)")
+    _need(tuple(positions.shape) in ((N,), (B, N)), f"{what}: positions {tuple(positions.shape)} are not [N] or [B, N] = {(B, N)}")
+    _need(eps > 0, f"{what}: eps {eps}")
+    for w in (q_weight, k_weight):
+        _need(w is None or (tuple(w.shape) == (D,) and w.is_floating_point()), f"{what}: a weight is not a floating [{D}]")
+    _need(not frequencies.requires_grad, f"{what}: no gradient to frequencies is built")
+    _on_device(what, q.device, k, q_weight, k_weight, positions, frequencies)
+    if positions.dim() == 1:
+        positions = positions.expand(B, N)
+    q_weight = q_weight.float().contiguous() if q_weight is not None else None
+    k_weight = k_weight.float().contiguous() if k_weight is not None else None
+    return _QkNormRope.apply(_rows(q), _rows(k), q_weight, k_weight, positions, frequencies.contiguous(), float(eps), bool(interleaved))
+
+
+# ---- attention ------------------------------------------------------------------------------------------------------------
+
+def _att_args(q, k, v, slopes, prefix, documents, lengths, starts, causal, scale, softcap):
+    a = _lib.AttentionArgs()
+    B, Nq, Hq, D = q.shape
+    a.dtype, a.B, a.Nq, a.Nk, a.Hq, a.Hk, a.D = _ATT_TYPES[q.dtype], B, Nq, k.shape[1], Hq, k.shape[2], D
+    a.causal, a.scale, a.softcap = causal, scale, softcap
+    a.q, a.k, a.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
+    a.q_stride_b, a.q_stride_n, a.q_stride_h = q.stride()[:3]
+    a.k_stride_b, a.k_stride_n, a.k_stride_h = k.stride()[:3]
+    a.v_stride_b, a.v_stride_n, a.v_stride_h = v.stride()[:3]
+    if slopes is not None:
+        a.slopes = slopes.data_ptr()
+    if prefix is not None:
+        a.prefix = prefix.data_ptr()
+    if lengths is not None:
+        a.lengths = lengths.data_ptr()
+    if starts is not None:
+        a.starts = starts.data_ptr()
+    if documents is not None:
+        a.documents, a.documents_stride = documents.data_ptr(), documents.stride(0)
+    return a
+
+
+def _att_forward(a, q, lse):
+    lib = _lib.load()
+    o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    a.o = o.data_ptr()
+    if lse is not None:
+        a.lse = lse.data_ptr()
+    with _Device(q.device) as stream:
+        own, ws, n = _workspace(lib.adk_attention_workspace(C.byref(a), 0), q.device)
+        _lib.check(lib.adk_attention(C.byref(a), ws, n, stream), "masked_attention")
+    return o
+
+
+class _MaskedAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, slopes, prefix, documents, lengths, starts, causal, scale, softcap):
+        a = _att_args(q, k, v, slopes, prefix, documents, lengths, starts, causal, scale, softcap)
+        lse = torch.empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32, device=q.device)
+        o = _att_forward(a, q, lse)
+        ctx.save_for_backward(q, k, v, slopes, prefix, documents, lengths, starts, o, lse)
+        ctx.how = (causal, scale, softcap)
+        return o
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, go):
+        q, k, v, slopes, prefix, documents, lengths, starts, o, lse = ctx.saved_tensors
+        a = _att_args(q, k, v, slopes, prefix, documents, lengths, starts, *ctx.how)
+        go = _rows16(go)
+        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+        a.o, a.lse, a.o_grad = o.data_ptr(), lse.data_ptr(), go.data_ptr()
+        a.og_stride_b, a.og_stride_n, a.og_stride_h = go.stride()[:3]
+        a.q_grad, a.k_grad, a.v_grad = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
+        if q.numel() == 0:
+            dk.zero_(), dv.zero_()
+        else:
+            lib = _lib.load()
+            with _Device(q.device) as stream:
+                own, ws, n = _workspace(lib.adk_attention_workspace(C.byref(a), 1), q.device)
+                _lib.check(lib.adk_attention_backward(C.byref(a), ws, n, stream), "masked_attention backward")
+        return dq, dk, dv, None, None, None, None, None, None, None, None
+
+
+def _index_tensor(what, name, t, shape):
+    _need(t.dtype == torch.int32 and tuple(t.shape) == shape, f"{what}: {name} is {t.dtype} {tuple(t.shape)}, must be int32 {list(shape)}")
+    return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
+
+
+def masked_attention(q, k, v, *, scale=None, softcap=None, slopes=None, causal=False, prefix=None, documents=None, lengths=None,
+                     starts=None):
+    """softmax(scores) v for ``q`` [B, Nq, Hq, D], ``k`` and ``v`` [B, Nk, Hk, D]; returns a new contiguous [B, Nq, Hq, D].
+
+    Query head h reads key head h // (Hq // Hk).  Query row i of sample b stands at position p = starts[b] + i (without
+    ``starts``: Nk - Nq + i, the last rows of the keys), key j at position j.
+
+    * ``scale``: of the products, default D ** -0.5.  ``softcap`` c: scores become c tanh(score / c).
+    * ``slopes`` float32 [Hq]: slopes[h] |p - j| is taken off the scores (``alibi_slopes``; constants, no gradient).
+    * ``causal``: row i sees j <= p.  ``prefix`` int32 [B] (with causal): and every j < prefix[b].
+    * ``lengths`` int32 [B]: keys j >= lengths[b] do not exist and are not read (values outside [0, Nk] are clamped).
+    * ``documents`` int32 [B, Nk]: row i sees keys of its own document, documents[b, p]; negative ids are padding, and
+      rows at a position outside [0, Nk) have no document.
+    A row that sees nothing gives zeros.  bfloat16 and float16, D = 32, 64 or 128, any strides (rows whose heads are not 16-byte
+    aligned are copied first).  Gradients flow to q, k and v, with a fixed summation order.  A single new token over a long
+    cache (Nq = 1) is split over the keys.
+    """
+    what = "masked_attention"
+    _need(q.dim() == 4 and k.dim() == 4 and k.shape == v.shape and q.shape[0] == k.shape[0] and q.shape[3] == k.shape[3],
+          f"{what}: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)} are not [B, Nq, Hq, D], [B, Nk, Hk, D] twice")
+    _need(q.dtype in _ATT_TYPES and k.dtype == q.dtype and v.dtype == q.dtype,
+          f"{what}: q is {q.dtype}, k {k.dtype}, v {v.dtype} (bfloat16 or float16, all alike)")
+    B, Nq, Hq, D = q.shape
+    Nk, Hk = k.shape[1:3]
+    _need(D in (32, 64, 128), f"{what}: head dim {D} (32, 64 or 128)")
+    _need(Hk >= 1 and Hq >= 1 and Hq % Hk == 0, f"{what}: {Hq} query heads are not a multiple of {Hk} key heads")
+    scale = D ** -0.5 if scale is None else float(scale)
+    softcap = 0.0 if softcap is None else float(softcap)
+    _need(scale > 0 and math.isfinite(scale), f"{what}: scale {scale} must be positive and finite")
+    _need(softcap >= 0 and math.isfinite(softcap), f"{what}: softcap {softcap} must be positive and finite")
+    _need(causal or prefix is None, f"{what}: prefix widens a causal mask: pass causal=True")
+    _on_device(what, q.device, k, v, slopes, prefix, documents, lengths, starts)
+    if slopes is not None:
+        _need(slopes.dtype == torch.float32 and tuple(slopes.shape) == (Hq,), f"{what}: slopes are {slopes.dtype} {tuple(slopes.shape)}, must be float32 [{Hq}]")
+        _need(not slopes.requires_grad, f"{what}: slopes are constants; no gradient to them is built")
+        slopes = slopes.contiguous()
+    prefix = None if prefix is None else _index_tensor(what, "prefix", prefix, (B,))
+    lengths = None if lengths is None else _index_tensor(what, "lengths", lengths, (B,))
+    starts = None if starts is None else _index_tensor(what, "starts", starts, (B,))
+    documents = None if documents is None else _index_tensor(what, "documents", documents, (B, Nk))
+    q, k, v = _rows16(q), _rows16(k), _rows16(v)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return _MaskedAttention.apply(q, k, v, slopes, prefix, documents, lengths, starts, int(causal), scale, softcap)
+    return _att_forward(_att_args(q, k, v, slopes, prefix, documents, lengths, starts, int(causal), scale, softcap), q, None)

@@ -295,6 +295,78 @@ int adk_group_norm_noalloc(int dtype, uint32_t flags, int B, int L, int P, int C
                            const void *x, const float *gamma, const float *beta, const void *residual, void *y,
                            void *stream);
 
+/* ---- operators on token sequences: rows [B, N, H, D], any strides, the D elements of a head contiguous -------------------
+ *
+ * Unlike the ops above these take their tensors in the layout of a linear projection's output (q, k, v may be views of one
+ * packed projection), not in CPL.  Strides are in ELEMENTS; outputs are contiguous [B, N, H, D].  A binding checks
+ * adk_sizeof_qk_norm_rope() / adk_sizeof_attention() against its mirror of the structs. */
+
+/* RMS norm of every query and key head and the position rotation in one pass (the qk-norm and rotary embedding in front of
+ * the attention of a transformer denoiser):
+ *   u = x / sqrt(mean_d x^2 + eps) * weight;   pair p of u turned by positions[b][n] * frequencies[p], p < R / 2,
+ *   pairs (p, p + R/2), or (2p, 2p + 1) with interleaved; elements R .. D - 1 are normed only.
+ * Angles are reduced in 64 bits, so far (and negative) positions keep their precision. */
+typedef struct adk_qk_norm_rope_args {
+    int32_t dtype;                       /* ADK_F32, ADK_BF16, ADK_F16: q, k, outputs and gradients                        */
+    int32_t B, N, Hq, Hk, D, R;          /* D even, 2 .. 256; R even, 0 .. D                                               */
+    int32_t interleaved;
+    int32_t pos_bytes;                   /* 4: int32 positions, 8: int64                                                   */
+    float eps;                           /* > 0                                                                            */
+    const void *q, *k;
+    int64_t q_stride_b, q_stride_n, q_stride_h, k_stride_b, k_stride_n, k_stride_h;
+    const float *q_weight, *k_weight;    /* f32 [D], or NULL: ones                                                         */
+    const void *positions;               /* [B, N], read at b * pos_stride_b + n * pos_stride_n (0: shared)                */
+    int64_t pos_stride_b, pos_stride_n;
+    const double *frequencies;           /* f64 [R / 2], radians per position                                              */
+    void *q_out, *k_out;                 /* forward: the results; backward: the gradients of q and k                       */
+    /* backward only */
+    const void *q_grad, *k_grad;         /* gradients of the two results                                                   */
+    int64_t qg_stride_b, qg_stride_n, qg_stride_h, kg_stride_b, kg_stride_n, kg_stride_h;
+    float *q_weight_grad, *k_weight_grad; /* f32 [D], or NULL: not wanted                                                  */
+} adk_qk_norm_rope_args;
+
+int adk_sizeof_qk_norm_rope(void);
+int adk_qk_norm_rope(const adk_qk_norm_rope_args *args, void *stream);
+/* bytes of workspace of the backward call (any contents, 16-byte aligned) */
+int64_t adk_qk_norm_rope_workspace(const adk_qk_norm_rope_args *args);
+int adk_qk_norm_rope_backward(const adk_qk_norm_rope_args *args, void *workspace, int64_t workspace_bytes, void *stream);
+
+/* Softmax attention with capped scores, a bias that depends on distance, and masks, without the score matrix in memory:
+ *   query row i of sample b stands at position p = starts[b] + i (starts NULL: Nk - Nq + i); key j at position j;
+ *   s = scale * q.k;   softcap > 0: s = softcap * tanh(s / softcap);   slopes: s -= slopes[h] * |p - j|;
+ *   row i sees key j if  j < lengths[b] (NULL: Nk)
+ *                   and  causal == 0, or j <= p, or j < prefix[b] (NULL: 0)
+ *                   and  documents NULL, or p in [0, Nk) and documents[b][p] == documents[b][j] >= 0;
+ *   o = softmax over the seen keys, times v.  A row that sees no key gives zeros (and no gradient).
+ * Query head h reads key head h / (Hq / Hk).  16-bit types; D = 32, 64 or 128; products of 16-bit values are summed in f32,
+ * probabilities are rounded to the type for the second product.  Keys at and past lengths[b] are not read. */
+typedef struct adk_attention_args {
+    int32_t dtype;                       /* ADK_BF16 or ADK_F16                                                            */
+    int32_t B, Nq, Nk, Hq, Hk, D;        /* Hq a multiple of Hk                                                            */
+    int32_t causal;
+    float scale, softcap;                /* scale > 0; softcap 0: none                                                     */
+    const void *q, *k, *v;               /* 16-byte aligned, strides multiples of 8 elements                               */
+    int64_t q_stride_b, q_stride_n, q_stride_h, k_stride_b, k_stride_n, k_stride_h, v_stride_b, v_stride_n, v_stride_h;
+    const float *slopes;                 /* f32 [Hq] or NULL                                                               */
+    const int32_t *prefix, *lengths, *starts;   /* int32 [B] or NULL                                                       */
+    const int32_t *documents;            /* int32 [B, Nk], rows documents_stride apart, or NULL; negative: padding         */
+    int64_t documents_stride;
+    void *o;                             /* [B, Nq, Hq, D]: forward: the result; backward: the forward's result            */
+    float *lse;                          /* f32 [B, Hq, Nq]: base-2 logarithm of the softmax sums (+inf: empty row); forward:
+                                            written unless NULL; backward: the forward's                                   */
+    /* backward only */
+    const void *o_grad;                  /* gradient of o, 16-byte aligned, strides multiples of 8 elements                */
+    int64_t og_stride_b, og_stride_n, og_stride_h;
+    void *q_grad, *k_grad, *v_grad;      /* [B, Nq, Hq, D], [B, Nk, Hk, D] twice                                           */
+} adk_attention_args;
+
+int adk_sizeof_attention(void);
+/* bytes of workspace of the forward (backward = 0) or backward call (any contents, 16-byte aligned; NULL if 0) */
+int64_t adk_attention_workspace(const adk_attention_args *args, int backward);
+int adk_attention(const adk_attention_args *args, void *workspace, int64_t workspace_bytes, void *stream);
+/* Gradients of q, k and v: fixed summation order, no atomics, the same bits on every run. */
+int adk_attention_backward(const adk_attention_args *args, void *workspace, int64_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
