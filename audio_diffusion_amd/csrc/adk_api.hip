@@ -619,6 +619,9 @@ static int check_att(const AttArgs* a, bool grad, const char* what)
     REQUIRE(al(a->q) && al(a->k) && al(a->v) && al(a->o), "%s: q, k, v and o must be 16-byte aligned", what);
     REQUIRE(s8(a->q_stride_b, a->q_stride_n, a->q_stride_h) && s8(a->k_stride_b, a->k_stride_n, a->k_stride_h)
             && s8(a->v_stride_b, a->v_stride_n, a->v_stride_h), "%s: strides must be multiples of 8 elements", what);
+    auto row = [](int64_t s) { return s >= 0 && s <= (1 << 24); };
+    REQUIRE(row(a->q_stride_n) && row(a->k_stride_n) && row(a->v_stride_n) && (!grad || row(a->og_stride_n)),
+            "%s: a row stride is not in [0, 2^24] elements", what);
     if (grad) {
         REQUIRE(a->lse && a->o_grad && a->q_grad && (a->Nk == 0 || (a->k_grad && a->v_grad)), "%s: null tensor", what);
         REQUIRE(al(a->o_grad) && al(a->q_grad) && al(a->k_grad) && al(a->v_grad) && s8(a->og_stride_b, a->og_stride_n, a->og_stride_h),

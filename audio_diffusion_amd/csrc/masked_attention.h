@@ -123,33 +123,81 @@ template <int D> __device__ __forceinline__ int at_swz(int row)
     const int hi = (row >> hi_shift) & (D / 32 - 1), lo = (row >> 2) & 3;
     return (hi << 2) | lo;
 }
-__device__ __forceinline__ void at_dma16(const void* src, unsigned char* lds)
+// The DMA instructions are written out: hipcc orders every later LDS read it cannot tell apart behind the builtin's transfers
+// (an s_waitcnt vmcnt(0) in front of the transposed reads of the CURRENT tile, which waited for the next one), and does not put
+// that wait in front of a barrier, where it belongs.  at_landed() is that wait: every wave calls it in front of the barrier after
+// which the tile is read.  The statements have no register results, so nothing can be reused under a transfer in flight.
+__device__ __forceinline__ void at_scalars() { asm volatile("s_nop 4" ::: "memory"); }
+__device__ __forceinline__ uint32_t at_lds_addr(const unsigned char* lds) { return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) unsigned char*)lds; }
+template <int PLUS> __device__ __forceinline__ void at_dma16(const unsigned char* base, uint32_t offset, uint32_t lds)  // lane l: 16 bytes of base + offset to lds + PLUS + 16 l
 {
-    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
-                                     (__attribute__((address_space(3))) void*)lds, 16, 0, 0);
+    asm volatile("s_add_u32 m0, %0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" :: "s"(lds), "v"(offset), "s"(base), "i"(PLUS) : "memory", "m0", "scc");
 }
-// 64 ints, one per lane, to lds + 4 lane
-__device__ __forceinline__ void at_dma4(const void* src, unsigned char* lds)
+__device__ __forceinline__ void at_dma4(const void* src, uint32_t lds)             // lane l: 4 bytes to lds + 4 l
 {
-    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
-                                     (__attribute__((address_space(3))) void*)lds, 4, 0, 0);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" :: "s"(lds), "v"(src) : "memory", "m0");
 }
-// ROWS x D rows starting at `row0` (rows past `last` repeat it) of a tensor with row stride `stride` elements; wave `wave`
-// of NW takes its share.  base points at row 0.
-template <int D, int ROWS, int NW>
-__device__ __forceinline__ void at_load_tile(const unsigned char* base, long long stride, int row0, int last, unsigned char* lds, int wave, int lane)
+// (The builtin, not asm: hipcc then knows that its own loads in front of the loop have landed too, and puts no wait for them
+// into the loop, where it would also wait for the tile in flight.)
+__device__ __forceinline__ void at_landed()
 {
-    constexpr int PPR = D / 8, RPI = 64 / PPR, NI = ROWS / RPI;          // pieces per row, rows per instruction
-    static_assert(NI % NW == 0, "every wave issues the same number of loads");
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x0f70);        // vmcnt(0), the other counters as they are
+    asm volatile("" ::: "memory");
+}
+// A barrier that orders LDS accesses in the program but waits for none of them (reads are consumed before their buffer is
+// asked for again, and DMA has its own wait).
+__device__ __forceinline__ void at_barrier()
+{
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+// Loads of 64-row tiles of two tensors x and y (K and V, or Q and dO), one tile behind the other in LDS.  Wave `wave` of NW issues
+// its share, the same number of instructions as every other, all of one tensor.  The 64-bit part of an address (first row of the
+// tile) is scalar and moves with the walk; a lane keeps the 32-bit offsets of its rows in the tile (64 rows of a 2^24-element stride at
+// most).  Scalar instructions take their turn in a wave's stream like any other: an address worked out afresh cost about 100 cycles per
+// request, as much as three products.
+template <int D, int NW> struct AtPair {
+    static constexpr int PPR = D / 8, RPI = 64 / PPR, NI = 64 / RPI, PER = 2 * NI / NW;  // pieces per row, rows per instruction
+    static_assert(2 * NI % NW == 0 && NI % PER == 0, "a wave's share lies in one tile");
+    const unsigned char* at;         // first row of the tile to ask for
+    long long step;                  // bytes of 64 rows
+    uint32_t stride, off[PER], lds;  // bytes of a row; per lane; the wave's part of a stage
+    int wave, lane;
+    __device__ __forceinline__ AtPair(const void* x, long long xs, const void* y, long long ys, uint32_t lds0, int wave_, int lane_) : wave(wave_), lane(lane_)
+    {
+        const bool second = wave * PER >= NI;
+        at = reinterpret_cast<const unsigned char*>(second ? y : x);
+        stride = (uint32_t)(second ? ys : xs) * 2;
+        step = (second ? ys : xs) * 128;
+        lds = lds0 + wave * PER * 1024;
 #pragma unroll
-    for (int t = 0; t < NI / NW; ++t) {
-        const int instr = wave * (NI / NW) + t;
-        const int row = instr * RPI + lane / PPR;
-        const int piece = (lane % PPR) ^ at_swz<D>(row);
-        const int gr = min(row0 + row, last);
-        at_dma16(base + ((long long)gr * stride + piece * 8) * 2, lds + instr * 1024);
+        for (int t = 0; t < PER; ++t) off[t] = (uint32_t)row(t) * stride + piece(t);
     }
-}
+    __device__ __forceinline__ int row(int t) const { return ((wave * PER + t) % NI) * RPI + lane / PPR; }
+    __device__ __forceinline__ uint32_t piece(int t) const { return ((lane % PPR) ^ at_swz<D>(row(t))) * 16; }
+    __device__ __forceinline__ void move(int tiles) { at += tiles * step; }
+    // the tile at hand holds rows 0 .. left of the tensor's last: rows past them repeat it.  Only ever the last tile of a walk.
+    __device__ __forceinline__ void clip(int left)
+    {
+        if (left < 63) {
+#pragma unroll
+            for (int t = 0; t < PER; ++t) off[t] = (uint32_t)min(row(t), left) * stride + piece(t);
+        }
+    }
+    // request I of PER into the stage at byte `stage`
+    template <int I> __device__ __forceinline__ void part(uint32_t stage) const
+    {
+        if constexpr (I < PER) at_dma16<I * 1024>(at, off[I], lds + stage);
+    }
+    __device__ __forceinline__ void load(uint32_t stage) const
+    {
+        at_scalars();
+        part<0>(stage); part<1>(stage); part<2>(stage); part<3>(stage);
+        part<4>(stage); part<5>(stage); part<6>(stage); part<7>(stage);
+    }
+};
 // Row fragment (A or B operand, contraction over d): lane (row = lane & 31, h) gets elements 16 ks + 8 h .. + 7 of row
 // row0 + (lane & 31).  `addr` = at_row_addr(lane), kept by the caller.
 template <int D> __device__ __forceinline__ int at_row_addr(int lane) { const int r = lane & 31; return r * 2 * D + (((lane >> 5) ^ at_swz<D>(r)) << 4); }
@@ -165,14 +213,32 @@ template <int D> __device__ __forceinline__ int at_tr_addr(int lane, int u)
     const int piece = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
     return r * 2 * D + ((piece ^ at_swz<D>(r)) << 4) + (lane & 1) * 8;
 }
+template <int D, typename Frag> union AtTr { att_s16x4 v[2]; Frag f; };
+// its half u, for reads that are spread out one by one
+template <int D> __device__ __forceinline__ att_s16x4 at_tr_half(const unsigned char* tile, const int (&addr)[2], int row0, int s, int dt, int u)
+{
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (__attribute__((address_space(3))) att_s16x4*)(tile + (row0 + 16 * s) * 2 * D + (addr[u] ^ (dt << 6))));
+}
 template <int D, typename Frag> __device__ __forceinline__ Frag at_tr_frag(const unsigned char* tile, const int (&addr)[2], int row0, int s, int dt)
 {
-    union { att_s16x4 v[2]; Frag f; } cv;
+    AtTr<D, Frag> cv;
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
-        cv.v[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (__attribute__((address_space(3))) att_s16x4*)(tile + (row0 + 16 * s) * 2 * D + (addr[u] ^ (dt << 6))));
+    for (int u = 0; u < 2; ++u) cv.v[u] = at_tr_half<D>(tile, addr, row0, s, dt, u);
     return cv.f;
+}
+
+// NM products with NR other instructions (LDS reads, mostly) spread between them, in exactly this order: an LDS instruction takes its
+// 16 or so cycles to issue while the matrix unit works on the product in front of it.  Issued in a bunch they leave it idle.
+template <int NM, int NR, typename F, typename R> __device__ __forceinline__ void at_weave(F product, R other)
+{
+#pragma unroll
+    for (int x = 0; x < NM; ++x) {
+        product(x);
+#pragma unroll
+        for (int r = x * NR / NM; r < (x + 1) * NR / NM; ++r) other(r);
+        __builtin_amdgcn_sched_barrier(0);
+    }
 }
 
 // 16 f32 -> two B operands (registers 0..7, 8..15)
@@ -193,8 +259,9 @@ template <typename T> __device__ __forceinline__ void at_pack(const f32x16& p, t
 template <int NW> struct AtWalk {
     const int* ranges;          // of the sample, or nullptr: no documents
     int t0, t1, lo, hi;
-    __device__ __forceinline__ int next(int t) const
+    __device__ __forceinline__ int next(int t) const       // t1 or more: none
     {
+        if (t >= t1) return t;
         ++t;
         if (ranges) while (t < t1 && !at_meet(at_range(ranges, t), lo, hi)) ++t;
         return t;
