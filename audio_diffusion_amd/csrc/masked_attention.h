@@ -139,10 +139,10 @@ __device__ __forceinline__ void at_dma4(const void* src, uint32_t lds)          
 }
 // (The builtin, not asm: hipcc then knows that its own loads in front of the loop have landed too, and puts no wait for them
 // into the loop, where it would also wait for the tile in flight.)
-__device__ __forceinline__ void at_landed()
+template <int YOUNGER = 0> __device__ __forceinline__ void at_landed()      // all but the YOUNGER last requests
 {
     asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_waitcnt(0x0f70);        // vmcnt(0), the other counters as they are
+    __builtin_amdgcn_s_waitcnt((YOUNGER & 15) | ((YOUNGER >> 4) << 14) | 0x0f70);        // vmcnt; the other counters as they are
     asm volatile("" ::: "memory");
 }
 // A barrier that orders LDS accesses in the program but waits for none of them (reads are consumed before their buffer is
@@ -290,6 +290,30 @@ __device__ __forceinline__ AtWalk<NW> at_walk(const AttArgs& a, const int* all_r
         w.lo = __builtin_amdgcn_readfirstlane(lo); w.hi = __builtin_amdgcn_readfirstlane(hi);
     }
     return w;
+}
+
+// ---- which forward kernel --------------------------------------------------------------------------------------------------
+// The step kernel splits keys over waves and blocks, the other one only query rows.  It takes over where most of a block's rows would be missing
+// (128 rows over 4096 keys, 32 heads of 64: 22 us, otherwise 58), and where those rows alone give too few blocks for 256 CUs.  bf16, step kernel /
+// the other: D = 128, 64 blocks (8 heads, 2048 rows) 46 / 56 us, 128 blocks (4096 rows) 152 / 104; D = 64, 128 blocks (2048 rows) 24 / 32 us, 256 blocks
+// (4096 rows) 83 / 64.
+// Its own blocks are split over the keys to fill the card once, at least 512 keys each (below that the joining costs more than it gains:
+// 4096 keys, 8 key heads of 128: 13.8 us, split to 256 keys 15.6) and, so that caches of unequal fill come out even, at most about 4096 (8 caches of 32 to
+// 64 Ki keys: 304 us, four splits of each 323).
+struct AtStepPlan { bool use; int nsplit; };
+static inline AtStepPlan at_step_plan(const AttArgs& a)
+{
+    const int rows = a.D == 128 ? 256 : 128;
+    const long long NR = (long long)a.Nq * (a.Hq / a.Hk), blocks = (long long)a.B * a.Hq * ((a.Nq + rows - 1) / rows);
+    AtStepPlan p = {blocks < (a.D == 128 ? 85 : 256) || a.Nq <= rows / 4, 1};
+    const long long items = (long long)a.B * a.Hk * ((NR + 31) / 32);
+    if (p.use && items > 0) {
+        const long long fill = 256 / items, even = items < 2048 ? a.Nk / 4096 : 0, most = a.Nk / 512;
+        long long n = fill > even ? fill : even;
+        n = n < most ? n : most;
+        p.nsplit = n < 1 ? 1 : (int)n;
+    }
+    return p;
 }
 
 // ---- launchers (one translation unit per type) -----------------------------------------------------------------------------

@@ -22,4 +22,8 @@ int att_launch_doc_ranges(const AttArgs& a, int* ranges, hipStream_t st)
     return hipGetLastError() == hipSuccess ? ADK_OK : ADK_ELAUNCH;
 }
 
-long long att_forward_workspace(const AttArgs& a) { return att_doc_bytes(a); }
+long long att_forward_workspace(const AttArgs& a)
+{
+    const AtStepPlan p = at_step_plan(a);
+    return att_doc_bytes(a) + (p.nsplit > 1 ? (long long)a.B * a.Nq * a.Hq * p.nsplit * (a.D + 2) * 4 : 0);
+}

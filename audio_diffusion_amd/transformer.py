@@ -32,15 +32,12 @@ def alibi_slopes(heads, device=None):
     return torch.exp2(-8.0 * torch.arange(1, heads + 1, dtype=torch.float64, device=device) / heads).float()
 
 
-def _need(ok, message, kind=ValueError):
-    if not ok:
-        raise kind(message)
-
-
 def _on_device(what, device, *tensors):
-    _need(device.type == "cuda", f"{what}: tensors are on {device}; there is no CPU path", RuntimeError)
+    if device.type != "cuda":
+        raise RuntimeError(f"{what}: tensors are on {device}; there is no CPU path")
     for t in tensors:
-        _need(t is None or t.device == device, f"{what}: tensors on {t.device if t is not None else ''} and {device}")
+        if t is not None and t.device != device:
+            raise ValueError(f"{what}: tensors on {t.device} and {device}")
 
 
 def _rows(t):
@@ -49,91 +46,77 @@ def _rows(t):
 
 
 def _rows16(t):
-    """Rows with 16-byte aligned heads (a copy if they are not)."""
+    """Rows with 16-byte aligned heads, at most 2^24 elements apart (a copy if they are not)."""
     sb, sn, sh, sd = t.stride()
-    if sd == 1 and not ((sb | sn | sh) & 7) and not (t.data_ptr() & 15):
+    if sd == 1 and not ((sb | sn | sh) & 7) and sn <= 1 << 24 and not (t.data_ptr() & 15):
         return t
     t = t.contiguous()
     return t if not (t.data_ptr() & 15) else t.clone()
 
 
-class _Device:
-    """Makes a device current for the launches of a call (a no-op where it is already)."""
-    __slots__ = ("want", "guard")
-
-    def __init__(self, device):
-        self.want, self.guard = device.index, None
-
-    def __enter__(self):
-        if torch.cuda.current_device() != self.want:
-            self.guard = torch.cuda.device(self.want)
-            self.guard.__enter__()
-        return C.c_void_p(torch.cuda.current_stream().cuda_stream)
-
-    def __exit__(self, *e):
-        if self.guard is not None:
-            self.guard.__exit__(*e)
-
-
-def _workspace(n, device):
-    """(tensor that owns it, pointer, bytes) of n bytes."""
-    if n <= 0:
-        return None, None, 0
-    w = torch.empty(n, dtype=torch.uint8, device=device)
-    return w, C.c_void_p(w.data_ptr()), n
+def _launch(what, device, entry, args, workspace_bytes=None):
+    """One library call on the device's current stream; with workspace_bytes (of the call's arguments) also its workspace, from
+    torch's allocator on that stream."""
+    if torch.cuda.current_device() != device.index:
+        with torch.cuda.device(device):
+            return _launch(what, device, entry, args, workspace_bytes)
+    stream = torch._C._cuda_getCurrentRawStream(device.index)
+    if workspace_bytes is None:
+        rc = entry(C.byref(args), stream)
+    elif workspace_bytes > 0:
+        w = torch.empty(workspace_bytes, dtype=torch.uint8, device=device)
+        rc = entry(C.byref(args), w.data_ptr(), workspace_bytes, stream)
+    else:
+        rc = entry(C.byref(args), None, 0, stream)
+    if rc:
+        _lib.check(rc, what)
 
 
 # ---- per-head norm and rotation -------------------------------------------------------------------------------------------
 
-def _norm_args(q, k, q_weight, k_weight, positions, frequencies, eps, interleaved):
+def _norm_args(q, k, q_weight, k_weight, positions, frequencies, eps, interleaved, q_out, k_out):
+    """QkNormRopeArgs in the order of its fields, up to the backward call's."""
     B, N, Hq, D = q.shape
-    a = _lib.QkNormRopeArgs()
-    a.dtype, a.B, a.N, a.Hq, a.Hk, a.D, a.R = _NORM_TYPES[q.dtype], B, N, Hq, k.shape[2], D, 2 * frequencies.shape[0]
-    a.interleaved, a.eps = int(interleaved), eps
-    a.q, a.k = q.data_ptr(), k.data_ptr()
-    a.q_stride_b, a.q_stride_n, a.q_stride_h = q.stride()[:3]
-    a.k_stride_b, a.k_stride_n, a.k_stride_h = k.stride()[:3]
-    a.q_weight = q_weight.data_ptr() if q_weight is not None else None
-    a.k_weight = k_weight.data_ptr() if k_weight is not None else None
-    a.pos_bytes, a.positions = positions.element_size(), positions.data_ptr()
-    a.pos_stride_b, a.pos_stride_n = positions.stride()
-    a.frequencies = frequencies.data_ptr()
-    return a
+    return _lib.QkNormRopeArgs(
+        _NORM_TYPES[q.dtype], B, N, Hq, k.shape[2], D, 2 * frequencies.shape[0], interleaved, positions.element_size(), eps,
+        q.data_ptr(), k.data_ptr(), *q.stride()[:3], *k.stride()[:3],
+        None if q_weight is None else q_weight.data_ptr(), None if k_weight is None else k_weight.data_ptr(), positions.data_ptr(),
+        *positions.stride(), frequencies.data_ptr(), q_out.data_ptr(), k_out.data_ptr())
+
+
+def _norm_forward(q, k, q_weight, k_weight, positions, frequencies, eps, interleaved):
+    qo, ko = torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(k.shape, dtype=k.dtype, device=q.device)
+    a = _norm_args(q, k, q_weight, k_weight, positions, frequencies, eps, interleaved, qo, ko)
+    _launch("qk_norm_rope", q.device, _lib.load().adk_qk_norm_rope, a)
+    return qo, ko
 
 
 class _QkNormRope(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, q_weight, k_weight, positions, frequencies, eps, interleaved):
-        a = _norm_args(q, k, q_weight, k_weight, positions, frequencies, eps, interleaved)
-        qo, ko = torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(k.shape, dtype=k.dtype, device=q.device)
-        a.q_out, a.k_out = qo.data_ptr(), ko.data_ptr()
-        with _Device(q.device) as stream:
-            _lib.check(_lib.load().adk_qk_norm_rope(C.byref(a), stream), "qk_norm_rope")
         ctx.save_for_backward(q, k, q_weight, k_weight, positions, frequencies)
         ctx.eps, ctx.interleaved = eps, interleaved
-        return qo, ko
+        return _norm_forward(q, k, q_weight, k_weight, positions, frequencies, eps, interleaved)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, gq, gk):
         q, k, q_weight, k_weight, positions, frequencies = ctx.saved_tensors
-        a = _norm_args(q, k, q_weight, k_weight, positions, frequencies, ctx.eps, ctx.interleaved)
         gq, gk = _rows(gq), _rows(gk)
         dq, dk = torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(k.shape, dtype=k.dtype, device=q.device)
-        a.q_out, a.k_out, a.q_grad, a.k_grad = dq.data_ptr(), dk.data_ptr(), gq.data_ptr(), gk.data_ptr()
-        a.qg_stride_b, a.qg_stride_n, a.qg_stride_h = gq.stride()[:3]
-        a.kg_stride_b, a.kg_stride_n, a.kg_stride_h = gk.stride()[:3]
         rows = q.shape[0] * q.shape[1]
         make = torch.empty_like if rows else torch.zeros_like
         dqw = make(q_weight) if q_weight is not None and ctx.needs_input_grad[2] else None
         dkw = make(k_weight) if k_weight is not None and ctx.needs_input_grad[3] else None
         if rows:
+            a = _norm_args(q, k, q_weight, k_weight, positions, frequencies, ctx.eps, ctx.interleaved, dq, dk)
+            a.q_grad, a.k_grad = gq.data_ptr(), gk.data_ptr()
+            a.qg_stride_b, a.qg_stride_n, a.qg_stride_h = gq.stride()[:3]
+            a.kg_stride_b, a.kg_stride_n, a.kg_stride_h = gk.stride()[:3]
             a.q_weight_grad = dqw.data_ptr() if dqw is not None else None
             a.k_weight_grad = dkw.data_ptr() if dkw is not None else None
             lib = _lib.load()
-            with _Device(q.device) as stream:
-                own, ws, n = _workspace(lib.adk_qk_norm_rope_workspace(C.byref(a)), q.device)
-                _lib.check(lib.adk_qk_norm_rope_backward(C.byref(a), ws, n, stream), "qk_norm_rope backward")
+            _launch("qk_norm_rope backward", q.device, lib.adk_qk_norm_rope_backward, a, lib.adk_qk_norm_rope_workspace(C.byref(a)))
         return dq, dk, dqw, dkw, None, None, None, None
 
 
@@ -149,70 +132,67 @@ def qk_norm_rope(q, k, q_weight, k_weight, positions, frequencies, eps=1e-6, int
     Gradients flow to q, k and the weights, not to positions or frequencies.
     """
     what = "qk_norm_rope"
-    _need(q.dim() == 4 and k.dim() == 4 and q.shape[:2] == k.shape[:2] and q.shape[3] == k.shape[3],
-          f"{what}: q {tuple(q.shape)} and k {tuple(k.shape)} are not [B, N, Hq, D] and [B, N, Hk, D]")
-    _need(q.dtype in _NORM_TYPES and k.dtype == q.dtype, f"{what}: q is {q.dtype}, k {k.dtype} (float32, bfloat16 or float16, both alike)")
+    if not (q.dim() == 4 and k.dim() == 4 and q.shape[:2] == k.shape[:2] and q.shape[3] == k.shape[3]):
+        raise ValueError(f"{what}: q {tuple(q.shape)} and k {tuple(k.shape)} are not [B, N, Hq, D] and [B, N, Hk, D]")
+    if not (q.dtype in _NORM_TYPES and k.dtype == q.dtype):
+        raise ValueError(f"{what}: q is {q.dtype}, k {k.dtype} (float32, bfloat16 or float16, both alike)")
     B, N, _, D = q.shape
-    _need(D % 2 == 0 and 2 <= D <= 256, f"{what}: head dim {D} is not even in [2, 256]")
-    _need(q.shape[2] >= 1 and k.shape[2] >= 1, f"{what}: no heads")
-    _need(frequencies.dim() == 1 and frequencies.dtype == torch.float64, f"{what}: frequencies must be float64 [R / 2]")
-    _need(2 * frequencies.shape[0] <= D, f"{what}: {frequencies.shape[0]} frequencies turn more than the {D} elements of a head")
-    _need(positions.dtype in (torch.int32, torch.int64), f"{what}: positions are {positions.dtype} (int32 or int64)")
-    _need(tuple(positions.shape) in ((N,), (B, N)), f"{what}: positions {tuple(positions.shape)} are not [N] or [B, N] = {(B, N)}")
-    _need(eps > 0, f"{what}: eps {eps}")
+    if not (D % 2 == 0 and 2 <= D <= 256):
+        raise ValueError(f"{what}: head dim {D} is not even in [2, 256]")
+    if not (q.shape[2] >= 1 and k.shape[2] >= 1):
+        raise ValueError(f"{what}: no heads")
+    if not (frequencies.dim() == 1 and frequencies.dtype == torch.float64):
+        raise ValueError(f"{what}: frequencies must be float64 [R / 2]")
+    if not (2 * frequencies.shape[0] <= D):
+        raise ValueError(f"{what}: {frequencies.shape[0]} frequencies turn more than the {D} elements of a head")
+    if not (positions.dtype in (torch.int32, torch.int64)):
+        raise ValueError(f"{what}: positions are {positions.dtype} (int32 or int64)")
+    if not (tuple(positions.shape) in ((N,), (B, N))):
+        raise ValueError(f"{what}: positions {tuple(positions.shape)} are not [N] or [B, N] = {(B, N)}")
+    if not (eps > 0):
+        raise ValueError(f"{what}: eps {eps}")
     for w in (q_weight, k_weight):
-        _need(w is None or (tuple(w.shape) == (D,) and w.is_floating_point()), f"{what}: a weight is not a floating [{D}]")
-    _need(not frequencies.requires_grad, f"{what}: no gradient to frequencies is built")
+        if not (w is None or (tuple(w.shape) == (D,) and w.is_floating_point())):
+            raise ValueError(f"{what}: a weight is not a floating [{D}]")
+    if frequencies.requires_grad:
+        raise ValueError(f"{what}: no gradient to frequencies is built")
     _on_device(what, q.device, k, q_weight, k_weight, positions, frequencies)
     if positions.dim() == 1:
         positions = positions.expand(B, N)
     q_weight = q_weight.float().contiguous() if q_weight is not None else None
     k_weight = k_weight.float().contiguous() if k_weight is not None else None
-    return _QkNormRope.apply(_rows(q), _rows(k), q_weight, k_weight, positions, frequencies.contiguous(), float(eps), bool(interleaved))
+    args = (_rows(q), _rows(k), q_weight, k_weight, positions, frequencies.contiguous(), float(eps), int(interleaved))
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:4]):
+        return _QkNormRope.apply(*args)
+    return _norm_forward(*args)
 
 
 # ---- attention ------------------------------------------------------------------------------------------------------------
 
-def _att_args(q, k, v, slopes, prefix, documents, lengths, starts, causal, scale, softcap):
-    a = _lib.AttentionArgs()
+def _att_args(q, k, v, slopes, prefix, documents, lengths, starts, causal, scale, softcap, o, lse):
+    """AttentionArgs in the order of its fields, up to the backward call's."""
     B, Nq, Hq, D = q.shape
-    a.dtype, a.B, a.Nq, a.Nk, a.Hq, a.Hk, a.D = _ATT_TYPES[q.dtype], B, Nq, k.shape[1], Hq, k.shape[2], D
-    a.causal, a.scale, a.softcap = causal, scale, softcap
-    a.q, a.k, a.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
-    a.q_stride_b, a.q_stride_n, a.q_stride_h = q.stride()[:3]
-    a.k_stride_b, a.k_stride_n, a.k_stride_h = k.stride()[:3]
-    a.v_stride_b, a.v_stride_n, a.v_stride_h = v.stride()[:3]
-    if slopes is not None:
-        a.slopes = slopes.data_ptr()
-    if prefix is not None:
-        a.prefix = prefix.data_ptr()
-    if lengths is not None:
-        a.lengths = lengths.data_ptr()
-    if starts is not None:
-        a.starts = starts.data_ptr()
-    if documents is not None:
-        a.documents, a.documents_stride = documents.data_ptr(), documents.stride(0)
-    return a
+    return _lib.AttentionArgs(
+        _ATT_TYPES[q.dtype], B, Nq, k.shape[1], Hq, k.shape[2], D, causal, scale, softcap, q.data_ptr(), k.data_ptr(), v.data_ptr(),
+        *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], None if slopes is None else slopes.data_ptr(),
+        None if prefix is None else prefix.data_ptr(), None if lengths is None else lengths.data_ptr(),
+        None if starts is None else starts.data_ptr(), None if documents is None else documents.data_ptr(),
+        0 if documents is None else documents.stride(0), o.data_ptr(), None if lse is None else lse.data_ptr())
 
 
-def _att_forward(a, q, lse):
+def _att_forward(q, k, v, slopes, prefix, documents, lengths, starts, causal, scale, softcap, lse=None):
     lib = _lib.load()
     o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    a.o = o.data_ptr()
-    if lse is not None:
-        a.lse = lse.data_ptr()
-    with _Device(q.device) as stream:
-        own, ws, n = _workspace(lib.adk_attention_workspace(C.byref(a), 0), q.device)
-        _lib.check(lib.adk_attention(C.byref(a), ws, n, stream), "masked_attention")
+    a = _att_args(q, k, v, slopes, prefix, documents, lengths, starts, causal, scale, softcap, o, lse)
+    _launch("masked_attention", q.device, lib.adk_attention, a, lib.adk_attention_workspace(C.byref(a), 0))
     return o
 
 
 class _MaskedAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, slopes, prefix, documents, lengths, starts, causal, scale, softcap):
-        a = _att_args(q, k, v, slopes, prefix, documents, lengths, starts, causal, scale, softcap)
         lse = torch.empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32, device=q.device)
-        o = _att_forward(a, q, lse)
+        o = _att_forward(q, k, v, slopes, prefix, documents, lengths, starts, causal, scale, softcap, lse)
         ctx.save_for_backward(q, k, v, slopes, prefix, documents, lengths, starts, o, lse)
         ctx.how = (causal, scale, softcap)
         return o
@@ -221,24 +201,22 @@ class _MaskedAttention(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, go):
         q, k, v, slopes, prefix, documents, lengths, starts, o, lse = ctx.saved_tensors
-        a = _att_args(q, k, v, slopes, prefix, documents, lengths, starts, *ctx.how)
-        go = _rows16(go)
         dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-        a.o, a.lse, a.o_grad = o.data_ptr(), lse.data_ptr(), go.data_ptr()
-        a.og_stride_b, a.og_stride_n, a.og_stride_h = go.stride()[:3]
-        a.q_grad, a.k_grad, a.v_grad = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
         if q.numel() == 0:
             dk.zero_(), dv.zero_()
         else:
+            go = _rows16(go)
+            a = _att_args(q, k, v, slopes, prefix, documents, lengths, starts, *ctx.how, o, lse)
+            a.o_grad, a.q_grad, a.k_grad, a.v_grad = go.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
+            a.og_stride_b, a.og_stride_n, a.og_stride_h = go.stride()[:3]
             lib = _lib.load()
-            with _Device(q.device) as stream:
-                own, ws, n = _workspace(lib.adk_attention_workspace(C.byref(a), 1), q.device)
-                _lib.check(lib.adk_attention_backward(C.byref(a), ws, n, stream), "masked_attention backward")
+            _launch("masked_attention backward", q.device, lib.adk_attention_backward, a, lib.adk_attention_workspace(C.byref(a), 1))
         return dq, dk, dv, None, None, None, None, None, None, None, None
 
 
 def _index_tensor(what, name, t, shape):
-    _need(t.dtype == torch.int32 and tuple(t.shape) == shape, f"{what}: {name} is {t.dtype} {tuple(t.shape)}, must be int32 {list(shape)}")
+    if not (t.dtype == torch.int32 and tuple(t.shape) == shape):
+        raise ValueError(f"{what}: {name} is {t.dtype} {tuple(t.shape)}, must be int32 {list(shape)}")
     return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
 
 
@@ -260,29 +238,36 @@ def masked_attention(q, k, v, *, scale=None, softcap=None, slopes=None, causal=F
     cache (Nq = 1) is split over the keys.
     """
     what = "masked_attention"
-    _need(q.dim() == 4 and k.dim() == 4 and k.shape == v.shape and q.shape[0] == k.shape[0] and q.shape[3] == k.shape[3],
-          f"{what}: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)} are not [B, Nq, Hq, D], [B, Nk, Hk, D] twice")
-    _need(q.dtype in _ATT_TYPES and k.dtype == q.dtype and v.dtype == q.dtype,
-          f"{what}: q is {q.dtype}, k {k.dtype}, v {v.dtype} (bfloat16 or float16, all alike)")
+    if not (q.dim() == 4 and k.dim() == 4 and k.shape == v.shape and q.shape[0] == k.shape[0] and q.shape[3] == k.shape[3]):
+        raise ValueError(f"{what}: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)} are not [B, Nq, Hq, D], [B, Nk, Hk, D] twice")
+    if not (q.dtype in _ATT_TYPES and k.dtype == q.dtype and v.dtype == q.dtype):
+        raise ValueError(f"{what}: q is {q.dtype}, k {k.dtype}, v {v.dtype} (bfloat16 or float16, all alike)")
     B, Nq, Hq, D = q.shape
     Nk, Hk = k.shape[1:3]
-    _need(D in (32, 64, 128), f"{what}: head dim {D} (32, 64 or 128)")
-    _need(Hk >= 1 and Hq >= 1 and Hq % Hk == 0, f"{what}: {Hq} query heads are not a multiple of {Hk} key heads")
+    if not (D in (32, 64, 128)):
+        raise ValueError(f"{what}: head dim {D} (32, 64 or 128)")
+    if not (Hk >= 1 and Hq >= 1 and Hq % Hk == 0):
+        raise ValueError(f"{what}: {Hq} query heads are not a multiple of {Hk} key heads")
     scale = D ** -0.5 if scale is None else float(scale)
     softcap = 0.0 if softcap is None else float(softcap)
-    _need(scale > 0 and math.isfinite(scale), f"{what}: scale {scale} must be positive and finite")
-    _need(softcap >= 0 and math.isfinite(softcap), f"{what}: softcap {softcap} must be positive and finite")
-    _need(causal or prefix is None, f"{what}: prefix widens a causal mask: pass causal=True")
+    if not (scale > 0 and math.isfinite(scale)):
+        raise ValueError(f"{what}: scale {scale} must be positive and finite")
+    if not (softcap >= 0 and math.isfinite(softcap)):
+        raise ValueError(f"{what}: softcap {softcap} must be positive and finite")
+    if not (causal or prefix is None):
+        raise ValueError(f"{what}: prefix widens a causal mask: pass causal=True")
     _on_device(what, q.device, k, v, slopes, prefix, documents, lengths, starts)
     if slopes is not None:
-        _need(slopes.dtype == torch.float32 and tuple(slopes.shape) == (Hq,), f"{what}: slopes are {slopes.dtype} {tuple(slopes.shape)}, must be float32 [{Hq}]")
-        _need(not slopes.requires_grad, f"{what}: slopes are constants; no gradient to them is built")
+        if not (slopes.dtype == torch.float32 and tuple(slopes.shape) == (Hq,)):
+            raise ValueError(f"{what}: slopes are {slopes.dtype} {tuple(slopes.shape)}, must be float32 [{Hq}]")
+        if slopes.requires_grad:
+            raise ValueError(f"{what}: slopes are constants; no gradient to them is built")
         slopes = slopes.contiguous()
     prefix = None if prefix is None else _index_tensor(what, "prefix", prefix, (B,))
     lengths = None if lengths is None else _index_tensor(what, "lengths", lengths, (B,))
     starts = None if starts is None else _index_tensor(what, "starts", starts, (B,))
     documents = None if documents is None else _index_tensor(what, "documents", documents, (B, Nk))
-    q, k, v = _rows16(q), _rows16(k), _rows16(v)
+    args = (_rows16(q), _rows16(k), _rows16(v), slopes, prefix, documents, lengths, starts, int(causal), scale, softcap)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        return _MaskedAttention.apply(q, k, v, slopes, prefix, documents, lengths, starts, int(causal), scale, softcap)
-    return _att_forward(_att_args(q, k, v, slopes, prefix, documents, lengths, starts, int(causal), scale, softcap), q, None)
+        return _MaskedAttention.apply(*args)
+    return _att_forward(*args)
