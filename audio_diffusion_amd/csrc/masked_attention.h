@@ -127,6 +127,9 @@ template <int D> __device__ __forceinline__ int at_swz(int row)
 // (an s_waitcnt vmcnt(0) in front of the transposed reads of the CURRENT tile, which waited for the next one), and does not put
 // that wait in front of a barrier, where it belongs.  at_landed() is that wait: every wave calls it in front of the barrier after
 // which the tile is read.  The statements have no register results, so nothing can be reused under a transfer in flight.
+// Program order of memory accesses, no instruction.  (Not an empty asm statement: hipcc counts every asm statement as a wait state behind a
+// matrix instruction, whatever it holds; statements below that only pin a value therefore hold an s_nop.)
+__device__ __forceinline__ void at_order() { __atomic_signal_fence(__ATOMIC_SEQ_CST); }
 __device__ __forceinline__ void at_scalars() { asm volatile("s_nop 4" ::: "memory"); }
 __device__ __forceinline__ uint32_t at_lds_addr(const unsigned char* lds) { return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) unsigned char*)lds; }
 template <int PLUS> __device__ __forceinline__ void at_dma16(const unsigned char* base, uint32_t offset, uint32_t lds)  // lane l: 16 bytes of base + offset to lds + PLUS + 16 l
@@ -141,17 +144,17 @@ __device__ __forceinline__ void at_dma4(const void* src, uint32_t lds)          
 // into the loop, where it would also wait for the tile in flight.)
 template <int YOUNGER = 0> __device__ __forceinline__ void at_landed()      // all but the YOUNGER last requests
 {
-    asm volatile("" ::: "memory");
+    at_order();
     __builtin_amdgcn_s_waitcnt((YOUNGER & 15) | ((YOUNGER >> 4) << 14) | 0x0f70);        // vmcnt; the other counters as they are
-    asm volatile("" ::: "memory");
+    at_order();
 }
 // A barrier that orders LDS accesses in the program but waits for none of them (reads are consumed before their buffer is
 // asked for again, and DMA has its own wait).
 __device__ __forceinline__ void at_barrier()
 {
-    asm volatile("" ::: "memory");
+    at_order();
     __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
+    at_order();
 }
 // Loads of 64-row tiles of two tensors x and y (K and V, or Q and dO), one tile behind the other in LDS.  Wave `wave` of NW issues
 // its share, the same number of instructions as every other, all of one tensor.  The 64-bit part of an address (first row of the
