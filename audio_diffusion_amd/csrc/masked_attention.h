@@ -134,11 +134,11 @@ __device__ __forceinline__ void at_scalars() { asm volatile("s_nop 4" ::: "memor
 __device__ __forceinline__ uint32_t at_lds_addr(const unsigned char* lds) { return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) unsigned char*)lds; }
 template <int PLUS> __device__ __forceinline__ void at_dma16(const unsigned char* base, uint32_t offset, uint32_t lds)  // lane l: 16 bytes of base + offset to lds + PLUS + 16 l
 {
-    asm volatile("s_add_u32 m0, %0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" :: "s"(lds), "v"(offset), "s"(base), "i"(PLUS) : "memory", "m0", "scc");
+    asm volatile("s_add_u32 m0, %0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" :: "s"(lds), "v"(offset), "s"(base), "i"(PLUS) : "memory", "scc");
 }
 __device__ __forceinline__ void at_dma4(const void* src, uint32_t lds)             // lane l: 4 bytes to lds + 4 l
 {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" :: "s"(lds), "v"(src) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" :: "s"(lds), "v"(src) : "memory");
 }
 // (The builtin, not asm: hipcc then knows that its own loads in front of the loop have landed too, and puts no wait for them
 // into the loop, where it would also wait for the tile in flight.)

@@ -91,7 +91,7 @@ def attention(q, k, v, *, scale=None, softcap=None, slopes=None, causal=False, p
     B, Nq, Hq, D = q.shape
     Nk, Hk = k.shape[1:3]
     G, dt, dev = Hq // Hk, q.dtype, q.device
-    u = torch.finfo(dt).eps / 2
+    u = torch.finfo(dt).eps / 2 if dt in (torch.bfloat16, torch.float16) else 0.0
     tiny = 2.0 ** -25 if dt == torch.float16 else UNDER
     scale = D ** -0.5 if scale is None else scale
     see, p = visible(B, Nq, Nk, dev, causal, prefix, documents, lengths, starts)

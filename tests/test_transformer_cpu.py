@@ -1,0 +1,151 @@
+"""CPU: what the token-sequence operators refuse, in the C ABI (before anything is launched) and in Python, their workspace sizes, and
+the structs' mirrors.  Pointers below are never followed."""
+import ctypes as C
+
+import pytest
+import torch
+
+import audio_diffusion_amd as A
+from audio_diffusion_amd import _lib
+
+P = 4096                                                     # a 16-byte aligned address that nothing reads
+
+
+def norm_args(**kw):
+    a = _lib.QkNormRopeArgs()
+    a.dtype, a.B, a.N, a.Hq, a.Hk, a.D, a.R, a.pos_bytes, a.eps = 1, 2, 3, 4, 2, 64, 32, 8, 1e-6
+    a.q = a.k = a.q_out = a.k_out = a.positions = a.frequencies = a.q_grad = a.k_grad = P
+    for n, v in kw.items():
+        setattr(a, n, v)
+    return a
+
+
+def att_args(**kw):
+    a = _lib.AttentionArgs()
+    a.dtype, a.B, a.Nq, a.Nk, a.Hq, a.Hk, a.D, a.scale = 1, 2, 30, 40, 4, 2, 64, 0.125
+    a.q = a.k = a.v = a.o = a.lse = a.o_grad = a.q_grad = a.k_grad = a.v_grad = P
+    a.q_stride_b, a.q_stride_n, a.q_stride_h = 30 * 256, 256, 64
+    a.k_stride_b, a.k_stride_n, a.k_stride_h = 40 * 128, 128, 64
+    a.v_stride_b, a.v_stride_n, a.v_stride_h = 40 * 128, 128, 64
+    a.og_stride_b, a.og_stride_n, a.og_stride_h = 30 * 256, 256, 64
+    for n, v in kw.items():
+        setattr(a, n, v)
+    return a
+
+
+def refused(rc, words):
+    assert rc == -1
+    text = _lib.load().adk_last_error().decode()
+    assert words in text, text
+
+
+def test_struct_sizes():
+    lib = _lib.load()
+    assert lib.adk_sizeof_qk_norm_rope() == C.sizeof(_lib.QkNormRopeArgs)
+    assert lib.adk_sizeof_attention() == C.sizeof(_lib.AttentionArgs)
+
+
+@pytest.mark.parametrize("kw, words", [
+    (dict(dtype=7), "dtype"), (dict(B=-1), "B=-1"), (dict(B=1 << 20, N=1 << 20), "2^31"), (dict(Hq=0), "heads"), (dict(Hk=1 << 20), "heads"),
+    (dict(D=65), "head dim"), (dict(D=258), "head dim"), (dict(D=0), "head dim"), (dict(R=33), "R=33"), (dict(R=66), "R=66"), (dict(R=-2), "R=-2"),
+    (dict(eps=0.0), "eps"), (dict(eps=float("nan")), "eps"), (dict(pos_bytes=2), "positions"), (dict(q=None), "null"), (dict(positions=None), "null"),
+    (dict(frequencies=None), "null"), (dict(k_out=None), "null"), (dict(q=P + 1), "aligned"), (dict(dtype=0, k=P + 2), "aligned")])
+def test_norm_refusals(kw, words):
+    lib = _lib.load()
+    refused(lib.adk_qk_norm_rope(C.byref(norm_args(**kw)), None), words)
+    refused(lib.adk_qk_norm_rope_backward(C.byref(norm_args(**kw)), C.c_void_p(P), 1 << 40, None), words)
+
+
+def test_norm_backward_refusals_and_workspace():
+    lib = _lib.load()
+    need = lib.adk_qk_norm_rope_workspace(C.byref(norm_args()))
+    assert need > 0 and lib.adk_qk_norm_rope_workspace(C.byref(norm_args(D=3))) == -1
+    refused(lib.adk_qk_norm_rope_backward(C.byref(norm_args()), None, need, None), "workspace")
+    refused(lib.adk_qk_norm_rope_backward(C.byref(norm_args()), C.c_void_p(P), need - 1, None), "workspace")
+    refused(lib.adk_qk_norm_rope_backward(C.byref(norm_args()), C.c_void_p(P + 4), need, None), "workspace")
+    refused(lib.adk_qk_norm_rope_backward(C.byref(norm_args(q_grad=None)), C.c_void_p(P), need, None), "gradient")
+    refused(lib.adk_qk_norm_rope_backward(C.byref(norm_args(B=0, q_weight_grad=P)), C.c_void_p(P), need, None), "weight gradient")
+    refused(lib.adk_qk_norm_rope(None, None), "null")
+    # nothing to do is no error, and nothing is read
+    assert lib.adk_qk_norm_rope(C.byref(norm_args(B=0, q=None)), None) == 0
+    assert lib.adk_qk_norm_rope_backward(C.byref(norm_args(N=0, q=None)), None, 0, None) == 0
+
+
+@pytest.mark.parametrize("kw, words", [
+    (dict(dtype=0), "dtype"), (dict(dtype=5), "dtype"), (dict(D=48), "head dim"), (dict(D=256), "head dim"), (dict(Hq=3), "multiple"), (dict(Hk=0), "multiple"),
+    (dict(Nq=-1), "Nq"), (dict(Nk=(1 << 28) + 1), "2^28"), (dict(B=70000), "grid"), (dict(B=60000, Hq=4096, Hk=4096, Nq=32000), "grid"),
+    (dict(scale=0.0), "scale"), (dict(scale=float("inf")), "scale"), (dict(scale=float("nan")), "scale"), (dict(softcap=-1.0), "softcap"),
+    (dict(softcap=float("nan")), "softcap"), (dict(prefix=P), "prefix"), (dict(q=None), "null"), (dict(v=None), "null"), (dict(o=None), "null"),
+    (dict(k=P + 2), "aligned"), (dict(o=P + 8), "aligned"), (dict(k_stride_h=60), "strides"), (dict(q_stride_n=(1 << 24) + 8), "2^24"), (dict(v_stride_n=-128), "2^24")])
+def test_attention_refusals(kw, words):
+    lib = _lib.load()
+    refused(lib.adk_attention(C.byref(att_args(**kw)), C.c_void_p(P), 1 << 40, None), words)
+    refused(lib.adk_attention_backward(C.byref(att_args(**kw)), C.c_void_p(P), 1 << 40, None), words)
+
+
+def test_attention_backward_refusals_and_workspaces():
+    lib = _lib.load()
+    assert lib.adk_attention_workspace(C.byref(att_args()), 0) == 0
+    docs = att_args(documents=P, documents_stride=40)
+    assert lib.adk_attention_workspace(C.byref(docs), 0) == 256
+    refused(lib.adk_attention(C.byref(docs), None, 0, None), "workspace")
+    # a long cache is split: f32 partial sums of every row and split
+    split = att_args(Nq=1, Nk=65536, B=1, Hq=8, Hk=2)
+    n = lib.adk_attention_workspace(C.byref(split), 0)
+    assert n > 0 and n % (8 * (64 + 2) * 4) == 0
+    refused(lib.adk_attention(C.byref(split), C.c_void_p(P), n - 1, None), "workspace")
+    need = lib.adk_attention_workspace(C.byref(att_args()), 1)
+    assert need >= 2 * 4 * 30 * 4
+    for kw, words in ((dict(lse=None), "null"), (dict(o_grad=None), "null"), (dict(k_grad=None), "null"), (dict(o_grad=P + 2), "aligned"), (dict(og_stride_n=4), "aligned"),
+                      (dict(og_stride_n=1 << 25), "2^24"), (dict(Nq=0), "no query rows")):
+        refused(lib.adk_attention_backward(C.byref(att_args(**kw)), C.c_void_p(P), need, None), words)
+    refused(lib.adk_attention_backward(C.byref(att_args()), C.c_void_p(P), need - 1, None), "workspace")
+    refused(lib.adk_attention(None, None, 0, None), "null")
+    assert lib.adk_attention_workspace(C.byref(att_args(D=1)), 0) == -1
+    for kw in (dict(B=0), dict(Nq=0)):
+        assert lib.adk_attention(C.byref(att_args(q=None, **kw)), None, 0, None) == 0
+        assert lib.adk_attention_workspace(C.byref(att_args(**kw)), 0) >= 0
+    assert lib.adk_attention_backward(C.byref(att_args(B=0)), None, 0, None) == 0
+
+
+def qkv(B=2, Nq=3, Nk=5, Hq=4, Hk=2, D=64, dtype=torch.bfloat16):
+    return torch.zeros(B, Nq, Hq, D, dtype=dtype), torch.zeros(B, Nk, Hk, D, dtype=dtype), torch.zeros(B, Nk, Hk, D, dtype=dtype)
+
+
+def test_python_refusals_attention():
+    q, k, v = qkv()
+    i32 = lambda *s: torch.zeros(s, dtype=torch.int32)                        # noqa: E731
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        A.masked_attention(q, k, v)
+    for args, kw, words in (((q[0], k, v), {}, "are not"), ((q, k, v[:, :4]), {}, "are not"), ((q, k[..., :32], v[..., :32]), {}, "are not"),
+                            ((q.float(), k.float(), v.float()), {}, "float32"), ((q, k.half(), v), {}, "alike"), (qkv(D=48), {}, "head dim"), (qkv(Hq=3), {}, "multiple"),
+                            ((q, k, v), dict(scale=-1.0), "scale"), ((q, k, v), dict(scale=float("nan")), "scale"), ((q, k, v), dict(softcap=-2), "softcap"),
+                            ((q, k, v), dict(prefix=i32(2)), "causal")):
+        with pytest.raises(ValueError, match=words):
+            A.masked_attention(*args, **kw)
+
+
+def test_python_refusals_norm():
+    q, k, _ = qkv(Nk=3)
+    pos, f = torch.arange(3), A.rope_frequencies(64)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        A.qk_norm_rope(q, k, None, None, pos, f)
+    w = torch.ones(64)
+    for args, kw, words in (((q, k[:, :2], None, None, pos, f), {}, "are not"), ((q.double(), k.double(), None, None, pos, f), {}, "float64"),
+                            ((q, k.half(), None, None, pos, f), {}, "alike"), ((q, k, None, None, pos.float(), f), {}, "positions"),
+                            ((q, k, None, None, pos[:2], f), {}, "positions"), ((q, k, None, None, pos, f.float()), {}, "float64"),
+                            ((q, k, None, None, pos, A.rope_frequencies(66)), {}, "more than"), ((q, k, w[:5], None, pos, f), {}, "weight"),
+                            ((q, k, None, w.int(), pos, f), {}, "weight"), ((q, k, None, None, pos, f), dict(eps=0), "eps"),
+                            ((q, k, None, None, pos, f.clone().requires_grad_()), {}, "frequencies")):
+        with pytest.raises(ValueError, match=words):
+            A.qk_norm_rope(*args, **kw)
+    with pytest.raises(ValueError):
+        A.rope_frequencies(7)
+
+
+def test_frequencies_and_slopes():
+    f = A.rope_frequencies(8, base=100.0)
+    assert f.dtype == torch.float64 and torch.allclose(f, torch.tensor([1.0, 100 ** -0.25, 0.1, 100 ** -0.75], dtype=torch.float64))
+    assert A.rope_frequencies(0).numel() == 0
+    s = A.alibi_slopes(4)
+    assert s.dtype == torch.float32 and s.tolist() == [0.25, 0.0625, 0.015625, 0.00390625]
