@@ -194,6 +194,14 @@ template <int D, int NW> struct AtPair {
     {
         if constexpr (I < PER) at_dma16<I * 1024>(at, off[I], lds + stage);
     }
+    // the same by a number that is known once its loop is unrolled
+    __device__ __forceinline__ void ask(int i, uint32_t stage) const
+    {
+        switch (i) {
+        case 0: return part<0>(stage); case 1: return part<1>(stage); case 2: return part<2>(stage); case 3: return part<3>(stage);
+        case 4: return part<4>(stage); case 5: return part<5>(stage); case 6: return part<6>(stage); default: return part<7>(stage);
+        }
+    }
     __device__ __forceinline__ void load(uint32_t stage) const
     {
         at_scalars();
