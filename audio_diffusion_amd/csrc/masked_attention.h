@@ -54,7 +54,7 @@ __device__ __forceinline__ AtSample at_sample(const AttArgs& a, int b)
     AtSample s;
     s.klen = a.lengths ? min(max(a.lengths[b], 0), a.Nk) : a.Nk;
     s.start = a.starts ? min(max(a.starts[b], -(1 << 29)), 1 << 29) : a.Nk - a.Nq;
-    s.prefix = a.prefix ? a.prefix[b] : 0;
+    s.prefix = a.prefix ? max(a.prefix[b], 0) : 0;
     return s;
 }
 __device__ __forceinline__ int at_limit(const AttArgs& a, const AtSample& s, int i)

@@ -339,7 +339,8 @@ int adk_qk_norm_rope_backward(const adk_qk_norm_rope_args *args, void *workspace
  *                   and  documents NULL, or p in [0, Nk) and documents[b][p] == documents[b][j] >= 0;
  *   o = softmax over the seen keys, times v.  A row that sees no key gives zeros (and no gradient).
  * Query head h reads key head h / (Hq / Hk).  16-bit types; D = 32, 64 or 128; products of 16-bit values are summed in f32,
- * probabilities are rounded to the type for the second product.  Keys at and past lengths[b] are not read. */
+ * probabilities are rounded to the type for the second product, and in the backward dS for its products.  Keys at and past
+ * lengths[b] are not read; starts, lengths and prefix may hold any int32.  Row strides (*_stride_n) lie in [0, 2^24]. */
 typedef struct adk_attention_args {
     int32_t dtype;                       /* ADK_BF16 or ADK_F16                                                            */
     int32_t B, Nq, Nk, Hq, Hk, D;        /* Hq a multiple of Hk                                                            */
@@ -352,8 +353,9 @@ typedef struct adk_attention_args {
     const int32_t *documents;            /* int32 [B, Nk], rows documents_stride apart, or NULL; negative: padding         */
     int64_t documents_stride;
     void *o;                             /* [B, Nq, Hq, D]: forward: the result; backward: the forward's result            */
-    float *lse;                          /* f32 [B, Hq, Nq]: base-2 logarithm of the softmax sums (+inf: empty row); forward:
-                                            written unless NULL; backward: the forward's                                   */
+    float *lse;                          /* f32 [B, Hq, Nq]: base-2 logarithm of the softmax sums (+inf: empty row; with slopes, rows
+                                            outside the keys: up to a constant of the row); forward: written unless NULL;
+                                            backward: the forward's                                                        */
     /* backward only */
     const void *o_grad;                  /* gradient of o, 16-byte aligned, strides multiples of 8 elements                */
     int64_t og_stride_b, og_stride_n, og_stride_h;

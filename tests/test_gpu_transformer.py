@@ -296,6 +296,64 @@ def test_attention_non_finite_values_in_hidden_places(A, case, dt):
     assert not bool(torch.isfinite(o[~before]).all(-1).any())
 
 
+SPLIT_CASES = {
+    # few keys under many rows: the keys' gradients are summed in parts
+    "heads": (1, 600, 130, 6, 2, 128, dict(causal=True)),
+    "heads of one": (2, 520, 200, 8, 1, 64, dict(slopes=True)),
+    "heads and rows": (1, 1400, 100, 4, 1, 128, {}),
+    "rows": (2, 2100, 70, 1, 1, 32, dict(softcap=10.0)),
+    "causal rows": (1, 2300, 2300, 2, 2, 64, dict(causal=True)),
+    "documents": (1, 1500, 1500, 4, 1, 128, dict(documents=300, causal=True, softcap=12.0)),
+    "all": (3, 1030, 1030, 6, 2, 64, dict(lengths=True, causal=True, prefix=True, documents=200, softcap=10.0, slopes=True)),
+    "lengths": (3, 1100, 1210, 3, 1, 32, dict(lengths=True, causal=True, starts=True)),
+}
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("name", SPLIT_CASES)
+def test_attention_gradients_in_parts(A, name, dt):
+    q, k, v, do, how = make(SPLIT_CASES[name], DT[dt], seed=3)
+    want = O.attention(q, k, v, grad=do, **how)
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    o = A.masked_attention(*leaves, **how)
+    grads = torch.autograd.grad(o, leaves, do, retain_graph=True)
+    for n, x in zip(("o", "dq", "dk", "dv"), (o,) + grads):
+        within(n, x, want[n])
+    assert all(torch.equal(x, y) for x, y in zip(grads, torch.autograd.grad(o, leaves, do)))
+
+
+def test_attention_gradients_in_parts_keep_non_finite_values_to_what_sees_them(A):
+    B, N, Hq, Hk, D = 1, 1400, 4, 1, 128
+    q, k, v, do, _ = make((B, N, N, Hq, Hk, D, {}), torch.bfloat16, seed=4)
+    docs = (torch.arange(N, device="cuda") * 3 // N).int()[None]
+    bad = docs == 1
+    want = O.attention(q, k, v, grad=do, documents=docs, causal=True)
+    g = gen(10)
+    leaves = [t.requires_grad_() for t in (poison(q, bad, g), poison(k, bad, g), poison(v, bad, g))]
+    o = A.masked_attention(*leaves, documents=docs, causal=True)
+    for n, x in zip(("o", "dq", "dk", "dv"), (o,) + torch.autograd.grad(o, leaves, poison(do, bad, g))):
+        within(n, x[~bad], tuple(t[~bad] for t in want[n]))
+
+
+def test_attention_extreme_mask_values(A):
+    """The ends of int32 in prefix, lengths and starts are values like any other."""
+    low, high = -2 ** 31, 2 ** 31 - 1
+    q, k, v, do, _ = make((2, 70, 70, 2, 1, 64, {}), torch.bfloat16)
+    i32 = lambda *x: torch.tensor(x, device="cuda", dtype=torch.int32)          # noqa: E731
+    for how, same in (
+        (dict(causal=True, prefix=i32(low, high)), dict(causal=True, prefix=i32(0, 70))),
+        (dict(lengths=i32(low, high)), dict(lengths=i32(0, 70))),
+        (dict(causal=True, starts=i32(low, high)), dict(causal=True, starts=i32(-70, 70))),
+        (dict(causal=True, starts=i32(low, high), prefix=i32(5, low)), dict(causal=True, starts=i32(-70, 70), prefix=i32(5, 0))),
+    ):
+        got = []
+        for h in (how, same):
+            leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+            o = A.masked_attention(*leaves, **h)
+            got.append((o.detach(),) + torch.autograd.grad(o, leaves, do) + (A.masked_attention(q[:, :1], k, v, **h),))
+        assert all(torch.equal(x, y) for x, y in zip(*got)), how
+
+
 def test_attention_layouts(A):
     """Views of one projection, other memory orders, unaligned and expanded tensors: the same bits as contiguous ones."""
     g = gen(3)
