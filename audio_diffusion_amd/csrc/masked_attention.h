@@ -112,6 +112,11 @@ __device__ __forceinline__ float at_tanh(float qk, float k1)
 {
     return 1.f - 2.f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(qk * k1) + 1.f);
 }
+// the capped score alone: cap tanh as one multiply-add of the reciprocal
+__device__ __forceinline__ float at_capped(float qk, const AtScore& sc)
+{
+    return __builtin_fmaf(-2.f * sc.capl2, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(qk * sc.k1) + 1.f), sc.capl2);
+}
 
 // ---- LDS tiles -----------------------------------------------------------------------------------------------------------
 // A tile is [rows][D] 16-bit, rows of 2 D bytes, filled by LDS-DMA (1 KiB per wave instruction, lane l at + 16 l).  Piece p
