@@ -64,6 +64,12 @@ __device__ __forceinline__ int at_limit(const AttArgs& a, const AtSample& s, int
 // The position a distance is taken from: outside the keys the distances differ from those of the nearest end by a constant
 // of the row, which the softmax does not see.
 __device__ __forceinline__ float at_bias_pos(const AttArgs& a, const AtSample& s, int i) { return (float)min(max(s.start + i, 0), a.Nk - 1); }
+// The bias -slope |pos - j| of a tile of 64 keys from k0 is side * (j - pos) where all keys stand on one side of the positions first .. last
+// (0: they do not, or there is no bias).
+__device__ __forceinline__ float at_side(float slope, int k0, float first, float last)
+{
+    return (float)(k0 + AT_KT - 1) <= first ? slope : (float)k0 >= last ? -slope : 0.f;
+}
 __device__ __forceinline__ int at_row_doc(const AttArgs& a, const AtSample& s, int b, int i)       // negative: none
 {
     const int p = s.start + i;
