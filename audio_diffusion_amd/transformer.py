@@ -5,7 +5,6 @@ They take rows ``[B, N, heads, head_dim]`` as a linear projection leaves them (v
 carry gradients.  Every call runs on the current stream of its tensors' device; outputs and workspaces come from torch's
 allocator on that stream, so a call can be captured in a graph.  No CPU or eager fallback.
 """
-import ctypes as C
 import math
 
 import torch
@@ -17,6 +16,18 @@ __all__ = ["qk_norm_rope", "rope_frequencies", "masked_attention", "alibi_slopes
 
 _NORM_TYPES = {torch.float32: _lib.ADK_F32, torch.bfloat16: _lib.ADK_BF16, torch.float16: _lib.ADK_F16}
 _ATT_TYPES = {torch.bfloat16: _lib.ADK_BF16, torch.float16: _lib.ADK_F16}
+_pack_norm, _pack_att = _lib.packer(_lib.QkNormRopeArgs), _lib.packer(_lib.AttentionArgs)
+_NO_GRADS = (0,) * 10                  # the backward fields of the norm's struct
+_NO_GRAD = (0,) * 7                    # and of the attention's
+
+
+def _ptr(t):
+    return 0 if t is None else t.data_ptr()
+
+
+def _like(t):
+    """New contiguous tensor of t's shape (a third of the time of torch.empty with its type and device)."""
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
 def rope_frequencies(rotary_dim, base=10000.0, device=None):
@@ -35,8 +46,9 @@ def alibi_slopes(heads, device=None):
 def _on_device(what, device, *tensors):
     if device.type != "cuda":
         raise RuntimeError(f"{what}: tensors are on {device}; there is no CPU path")
+    index = device.index
     for t in tensors:
-        if t is not None and t.device != device:
+        if t is not None and t.get_device() != index:          # -1 on the CPU
             raise ValueError(f"{what}: tensors on {t.device} and {device}")
 
 
@@ -55,37 +67,37 @@ def _rows16(t):
 
 
 def _launch(what, device, entry, args, workspace_bytes=None):
-    """One library call on the device's current stream; with workspace_bytes (of the call's arguments) also its workspace, from
-    torch's allocator on that stream."""
-    if torch.cuda.current_device() != device.index:
+    """One library call on the device's current stream; args are its struct's bytes; with workspace_bytes (of the call's arguments)
+    also its workspace, from torch's allocator on that stream."""
+    if torch._C._cuda_getDevice() != device.index:
         with torch.cuda.device(device):
             return _launch(what, device, entry, args, workspace_bytes)
     stream = torch._C._cuda_getCurrentRawStream(device.index)
     if workspace_bytes is None:
-        rc = entry(C.byref(args), stream)
+        rc = entry(args, stream)
     elif workspace_bytes > 0:
         w = torch.empty(workspace_bytes, dtype=torch.uint8, device=device)
-        rc = entry(C.byref(args), w.data_ptr(), workspace_bytes, stream)
+        rc = entry(args, w.data_ptr(), workspace_bytes, stream)
     else:
-        rc = entry(C.byref(args), None, 0, stream)
+        rc = entry(args, None, 0, stream)
     if rc:
         _lib.check(rc, what)
 
 
 # ---- per-head norm and rotation -------------------------------------------------------------------------------------------
 
-def _norm_args(q, k, q_weight, k_weight, positions, frequencies, eps, interleaved, q_out, k_out):
-    """QkNormRopeArgs in the order of its fields, up to the backward call's."""
+def _norm_args(q, k, q_weight, k_weight, positions, frequencies, eps, interleaved, q_out, k_out, grads=_NO_GRADS):
+    """QkNormRopeArgs in the order of its fields; grads: the backward call's."""
     B, N, Hq, D = q.shape
-    return _lib.QkNormRopeArgs(
+    return _pack_norm(
         _NORM_TYPES[q.dtype], B, N, Hq, k.shape[2], D, 2 * frequencies.shape[0], interleaved, positions.element_size(), eps,
         q.data_ptr(), k.data_ptr(), *q.stride()[:3], *k.stride()[:3],
-        None if q_weight is None else q_weight.data_ptr(), None if k_weight is None else k_weight.data_ptr(), positions.data_ptr(),
-        *positions.stride(), frequencies.data_ptr(), q_out.data_ptr(), k_out.data_ptr())
+        _ptr(q_weight), _ptr(k_weight), positions.data_ptr(), *positions.stride(), frequencies.data_ptr(), q_out.data_ptr(), k_out.data_ptr(),
+        *grads)
 
 
 def _norm_forward(q, k, q_weight, k_weight, positions, frequencies, eps, interleaved):
-    qo, ko = torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(k.shape, dtype=k.dtype, device=q.device)
+    qo, ko = _like(q), _like(k)
     a = _norm_args(q, k, q_weight, k_weight, positions, frequencies, eps, interleaved, qo, ko)
     _launch("qk_norm_rope", q.device, _lib.load().adk_qk_norm_rope, a)
     return qo, ko
@@ -103,20 +115,16 @@ class _QkNormRope(torch.autograd.Function):
     def backward(ctx, gq, gk):
         q, k, q_weight, k_weight, positions, frequencies = ctx.saved_tensors
         gq, gk = _rows(gq), _rows(gk)
-        dq, dk = torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(k.shape, dtype=k.dtype, device=q.device)
+        dq, dk = _like(q), _like(k)
         rows = q.shape[0] * q.shape[1]
         make = torch.empty_like if rows else torch.zeros_like
         dqw = make(q_weight) if q_weight is not None and ctx.needs_input_grad[2] else None
         dkw = make(k_weight) if k_weight is not None and ctx.needs_input_grad[3] else None
         if rows:
-            a = _norm_args(q, k, q_weight, k_weight, positions, frequencies, ctx.eps, ctx.interleaved, dq, dk)
-            a.q_grad, a.k_grad = gq.data_ptr(), gk.data_ptr()
-            a.qg_stride_b, a.qg_stride_n, a.qg_stride_h = gq.stride()[:3]
-            a.kg_stride_b, a.kg_stride_n, a.kg_stride_h = gk.stride()[:3]
-            a.q_weight_grad = dqw.data_ptr() if dqw is not None else None
-            a.k_weight_grad = dkw.data_ptr() if dkw is not None else None
+            a = _norm_args(q, k, q_weight, k_weight, positions, frequencies, ctx.eps, ctx.interleaved, dq, dk,
+                           (gq.data_ptr(), gk.data_ptr(), *gq.stride()[:3], *gk.stride()[:3], _ptr(dqw), _ptr(dkw)))
             lib = _lib.load()
-            _launch("qk_norm_rope backward", q.device, lib.adk_qk_norm_rope_backward, a, lib.adk_qk_norm_rope_workspace(C.byref(a)))
+            _launch("qk_norm_rope backward", q.device, lib.adk_qk_norm_rope_backward, a, lib.adk_qk_norm_rope_workspace(a))
         return dq, dk, dqw, dkw, None, None, None, None
 
 
@@ -169,22 +177,20 @@ def qk_norm_rope(q, k, q_weight, k_weight, positions, frequencies, eps=1e-6, int
 
 # ---- attention ------------------------------------------------------------------------------------------------------------
 
-def _att_args(q, k, v, slopes, prefix, documents, lengths, starts, causal, scale, softcap, o, lse):
-    """AttentionArgs in the order of its fields, up to the backward call's."""
+def _att_args(q, k, v, slopes, prefix, documents, lengths, starts, causal, scale, softcap, o, lse, grads=_NO_GRAD):
+    """AttentionArgs in the order of its fields; grads: the backward call's."""
     B, Nq, Hq, D = q.shape
-    return _lib.AttentionArgs(
+    return _pack_att(
         _ATT_TYPES[q.dtype], B, Nq, k.shape[1], Hq, k.shape[2], D, causal, scale, softcap, q.data_ptr(), k.data_ptr(), v.data_ptr(),
-        *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], None if slopes is None else slopes.data_ptr(),
-        None if prefix is None else prefix.data_ptr(), None if lengths is None else lengths.data_ptr(),
-        None if starts is None else starts.data_ptr(), None if documents is None else documents.data_ptr(),
-        0 if documents is None else documents.stride(0), o.data_ptr(), None if lse is None else lse.data_ptr())
+        *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], _ptr(slopes), _ptr(prefix), _ptr(lengths), _ptr(starts), _ptr(documents),
+        0 if documents is None else documents.stride(0), o.data_ptr(), _ptr(lse), *grads)
 
 
 def _att_forward(q, k, v, slopes, prefix, documents, lengths, starts, causal, scale, softcap, lse=None):
     lib = _lib.load()
-    o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    o = _like(q)
     a = _att_args(q, k, v, slopes, prefix, documents, lengths, starts, causal, scale, softcap, o, lse)
-    _launch("masked_attention", q.device, lib.adk_attention, a, lib.adk_attention_workspace(C.byref(a), 0))
+    _launch("masked_attention", q.device, lib.adk_attention, a, lib.adk_attention_workspace(a, 0))
     return o
 
 
@@ -201,16 +207,15 @@ class _MaskedAttention(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, go):
         q, k, v, slopes, prefix, documents, lengths, starts, o, lse = ctx.saved_tensors
-        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+        dq, dk, dv = _like(q), _like(k), _like(v)
         if q.numel() == 0:
             dk.zero_(), dv.zero_()
         else:
             go = _rows16(go)
-            a = _att_args(q, k, v, slopes, prefix, documents, lengths, starts, *ctx.how, o, lse)
-            a.o_grad, a.q_grad, a.k_grad, a.v_grad = go.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
-            a.og_stride_b, a.og_stride_n, a.og_stride_h = go.stride()[:3]
+            a = _att_args(q, k, v, slopes, prefix, documents, lengths, starts, *ctx.how, o, lse,
+                          (go.data_ptr(), *go.stride()[:3], dq.data_ptr(), dk.data_ptr(), dv.data_ptr()))
             lib = _lib.load()
-            _launch("masked_attention backward", q.device, lib.adk_attention_backward, a, lib.adk_attention_workspace(C.byref(a), 1))
+            _launch("masked_attention backward", q.device, lib.adk_attention_backward, a, lib.adk_attention_workspace(a, 1))
         return dq, dk, dv, None, None, None, None, None, None, None, None
 
 
