@@ -149,3 +149,15 @@ def test_frequencies_and_slopes():
     assert A.rope_frequencies(0).numel() == 0
     s = A.alibi_slopes(4)
     assert s.dtype == torch.float32 and s.tolist() == [0.25, 0.0625, 0.015625, 0.00390625]
+
+
+def test_packed_structs_have_the_mirrors_layout_and_cut_nothing_off():
+    for mirror in (_lib.QkNormRopeArgs, _lib.AttentionArgs):
+        pack = _lib.packer(mirror)
+        values = [float(n + 1) if t is C.c_float else n + 1 for n, (_, t) in enumerate(mirror._fields_)]
+        a = mirror.from_buffer_copy(pack(*values))
+        assert [getattr(a, name) for name, _ in mirror._fields_] == values
+        for n, (_, t) in enumerate(mirror._fields_):
+            if t in (C.c_int32, C.c_float):
+                with pytest.raises(ValueError, match="beyond"):
+                    pack(*values[:n], 1 << 31 if t is C.c_int32 else 1e39, *values[n + 1:])
