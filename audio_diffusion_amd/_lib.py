@@ -92,9 +92,10 @@ class AttentionArgs(C.Structure):
 
 def packer(mirror):
     """The struct's bytes from all of its fields in order (pointers as integers): a sixth of the time of filling a ctypes instance,
-    and sizes that do not fit raise ValueError instead of being cut off."""
-    codes = {C.c_int32: "i", C.c_int64: "q", C.c_float: "f", C.c_void_p: "P"}
-    layout = struct.Struct("@" + "".join(codes[t] for _, t in mirror._fields_))
+    and what does not fit its field raises ValueError instead of being cut off.  (Standard sizes: native ones take 1e39 for an infinity.
+    The structs need no padding.)"""
+    codes = {C.c_int32: "i", C.c_int64: "q", C.c_float: "f", C.c_void_p: "Q"}
+    layout = struct.Struct("<" + "".join(codes[t] for _, t in mirror._fields_))
     assert layout.size == C.sizeof(mirror)
 
     def pack(*fields):
