@@ -335,6 +335,30 @@ def test_attention_gradients_in_parts_keep_non_finite_values_to_what_sees_them(A
         within(n, x[~bad], tuple(t[~bad] for t in want[n]))
 
 
+KEY_SPLIT_CASES = {
+    # few rows over many keys: the queries' gradients are summed in parts
+    "whole": (1, 64, 2200, 4, 2, 128, {}),
+    "one row": (2, 1, 3000, 2, 1, 64, dict(slopes=True)),
+    "causal": (1, 300, 2300, 2, 2, 64, dict(causal=True, softcap=9.0)),
+    "documents": (2, 70, 1500, 3, 1, 128, dict(documents=300, causal=True)),
+    "lengths": (3, 40, 1300, 4, 2, 32, dict(lengths=True, causal=True, starts=True, slopes=True)),
+    "all": (2, 1100, 1100, 2, 1, 128, dict(lengths=True, causal=True, prefix=True, documents=250, softcap=10.0, slopes=True)),
+}
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("name", KEY_SPLIT_CASES)
+def test_attention_query_gradients_in_parts(A, name, dt):
+    q, k, v, do, how = make(KEY_SPLIT_CASES[name], DT[dt], seed=5)
+    want = O.attention(q, k, v, grad=do, **how)
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    o = A.masked_attention(*leaves, **how)
+    grads = torch.autograd.grad(o, leaves, do, retain_graph=True)
+    for n, x in zip(("o", "dq", "dk", "dv"), (o,) + grads):
+        within(n, x, want[n])
+    assert all(torch.equal(x, y) for x, y in zip(grads, torch.autograd.grad(o, leaves, do)))
+
+
 def test_attention_extreme_mask_values(A):
     """The ends of int32 in prefix, lengths and starts are values like any other."""
     low, high = -2 ** 31, 2 ** 31 - 1
