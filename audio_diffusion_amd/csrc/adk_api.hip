@@ -611,6 +611,8 @@ static int check_att(const AttArgs* a, bool grad, const char* what)
             && (long long)a->Nq * (a->Hq / a->Hk) < (1LL << 30), "%s: B=%d x heads %d / %d x rows %d / %d exceed the grid", what, a->B, a->Hq, a->Hk, a->Nq, a->Nk);
     REQUIRE(a->scale > 0.f && a->scale <= 3.0e38f, "%s: scale=%g must be positive and finite", what, (double)a->scale);
     REQUIRE(a->softcap >= 0.f && a->softcap <= 3.0e38f, "%s: softcap=%g must be positive and finite, or 0", what, (double)a->softcap);
+    REQUIRE(at_scores_finite(*a), "%s: scale=%g, softcap=%g: 1.45 scale, 2.89 scale / softcap and 2.89 softcap must be within the range of f32", what,
+            (double)a->scale, (double)a->softcap);
     REQUIRE(a->causal || !a->prefix, "%s: a prefix mask widens a causal one: set causal", what);
     if (a->B == 0 || a->Nq == 0) return ADK_OK;            // no rows
     REQUIRE(a->q && a->o && (a->Nk == 0 || (a->k && a->v)), "%s: null tensor", what);

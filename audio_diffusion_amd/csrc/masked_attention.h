@@ -6,6 +6,7 @@
 // rounded to 16 bits, are the B operand of the next product as they stand: neither scores nor probabilities touch LDS.
 #pragma once
 #include "adk_common.h"
+#include <cmath>
 
 typedef adk_attention_args AttArgs;
 typedef __attribute__((ext_vector_type(4))) short att_s16x4;
@@ -103,25 +104,68 @@ __device__ __forceinline__ AtRange at_range(const int* ranges, int t)
 __device__ __forceinline__ bool at_meet(const AtRange& r, int lo, int hi) { return r.lo <= hi && r.hi >= lo; }
 
 // ---- scores --------------------------------------------------------------------------------------------------------------
-// base-2 scores: x = score * log2(e).  Plain: x = qk * c.  Capped: c tanh(t) = c (1 - 2 / (exp(2 t) + 1)), t = qk * scale / cap.
-struct AtScore { float c, k1, capl2; };      // scale * log2 e;  2 log2 e scale / cap;  cap * log2 e
+// base-2 scores: x = score * log2(e).  Plain (CAP = 0): x = qk * c.  Capped: c tanh(t), t = qk * scale / cap, in two forms.
+//   CAP = 1, caps up to AT_NEAR_CAP: cap - 2 cap / (exp(2 t) + 1).  Its error is that of a difference of numbers as large as the cap: the
+//   exponential and the reciprocal are off by a step of 2^-23, the sums by half of one, 2.4e-7 cap of the score together, 3e-5 at most here.
+//   CAP = 2, larger caps: where |t| < 0.35 the Taylor series of tanh (to t^11; the next term is 1.2e-8 of the first), which multiplies the
+//   score and has an error relative to it; elsewhere the same difference, there 2.4e-7 cap < 7e-7 |score|.
+//   The second form has kernels of its own, since it takes longer (2 x 16 heads on 4 of 8192 x 8192 at D = 128, causal, bf16: forward 655 -> 1053 us,
+//   backward 2158 -> 2778).
+// Caps whose factors leave the range of f32 are refused (at_scores_finite).
+struct AtScore { float c, k1, capl2, t; };   // scale * log2 e;  2 log2 e scale / cap;  cap * log2 e;  scale / cap
 
+constexpr float AT_NEAR_CAP = 128.f;
+static inline int at_cap_of(const AttArgs& a) { return a.softcap == 0.f ? 0 : a.softcap <= AT_NEAR_CAP ? 1 : 2; }
 static inline AtScore at_score_of(const AttArgs& a)
 {
     AtScore s;
     s.c = a.scale * AT_LOG2E;
-    s.k1 = a.softcap > 0.f ? 2.f * AT_LOG2E * a.scale / a.softcap : 0.f;
+    s.k1 = a.softcap > 0.f ? 2.f * AT_LOG2E * (a.scale / a.softcap) : 0.f;
     s.capl2 = a.softcap * AT_LOG2E;
+    s.t = a.softcap > 0.f ? a.scale / a.softcap : 0.f;
     return s;
+}
+static inline bool at_scores_finite(const AttArgs& a)
+{
+    const AtScore s = at_score_of(a);
+    return std::isfinite(s.c) && std::isfinite(s.k1) && std::isfinite(2.f * s.capl2);
 }
 __device__ __forceinline__ float at_tanh(float qk, float k1)
 {
     return 1.f - 2.f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(qk * k1) + 1.f);
 }
-// the capped score alone: cap tanh as one multiply-add of the reciprocal
-__device__ __forceinline__ float at_capped(float qk, const AtScore& sc)
+// tanh(t) / t for |t| < 0.35
+__device__ __forceinline__ float at_tanh_series(float t)
 {
-    return __builtin_fmaf(-2.f * sc.capl2, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(qk * sc.k1) + 1.f), sc.capl2);
+    const float u = t * t;
+    float p = __builtin_fmaf(u, -1382.f / 155925.f, 62.f / 2835.f);
+    p = __builtin_fmaf(u, p, -17.f / 315.f);
+    p = __builtin_fmaf(u, p, 2.f / 15.f);
+    p = __builtin_fmaf(u, p, -1.f / 3.f);
+    return __builtin_fmaf(u, p, 1.f);
+}
+// a score less y, and the tanh for its derivative
+template <int CAP> __device__ __forceinline__ float at_score(const AtScore& sc, float qk, float y, float& th)
+{
+    if constexpr (CAP == 0) {
+        th = 0.f;
+        return __builtin_fmaf(qk, sc.c, -y);
+    } else if constexpr (CAP == 1) {
+        th = at_tanh(qk, sc.k1);
+        return __builtin_fmaf(th, sc.capl2, -y);
+    } else {
+        const float t = qk * sc.t, p = at_tanh_series(t), far = at_tanh(qk, sc.k1);
+        const bool near = fabsf(t) < 0.35f;
+        th = near ? t * p : far;
+        return __builtin_fmaf(near ? qk * sc.c : sc.capl2, near ? p : far, -y);
+    }
+}
+// the capped score alone: in the first form cap tanh as one multiply-add of the reciprocal
+template <int CAP> __device__ __forceinline__ float at_capped(float qk, const AtScore& sc)
+{
+    if constexpr (CAP == 1) return __builtin_fmaf(-2.f * sc.capl2, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(qk * sc.k1) + 1.f), sc.capl2);
+    float th;
+    return at_score<CAP>(sc, qk, 0.f, th);
 }
 
 // ---- LDS tiles -----------------------------------------------------------------------------------------------------------

@@ -34,10 +34,9 @@ template <typename T, int D> __device__ __forceinline__ float at_dot(const T* x,
     }
     return s;
 }
-template <bool CAP, bool BIAS> __device__ __forceinline__ float at_base2(const AtScore& sc, float qk, float slope2, float dist, float& th)
+template <int CAP, bool BIAS> __device__ __forceinline__ float at_base2(const AtScore& sc, float qk, float slope2, float dist, float& th)
 {
-    th = CAP ? at_tanh(qk, sc.k1) : 0.f;
-    float x = CAP ? sc.capl2 * th : qk * sc.c;
+    float x = at_score<CAP>(sc, qk, 0.f, th);
     if (BIAS) x = __builtin_fmaf(-slope2, fabsf(dist), x);
     return x;
 }
@@ -62,7 +61,7 @@ template <typename T> __device__ __forceinline__ AtOperands<T> at_operands(const
 }
 
 // forward: row i over the keys j0 .. j1 - 1 that it sees
-template <typename T, int D, bool CAP, bool BIAS>
+template <typename T, int D, int CAP, bool BIAS>
 __device__ __forceinline__ void at_exact_row(const AttArgs& a, const AtScore& sc, const AtSample& sm, int b, int head, int i, int j0, int j1,
                                              float& m, float& l, float (&o)[2])
 {
@@ -95,7 +94,7 @@ __device__ __forceinline__ void at_exact_row(const AttArgs& a, const AtScore& sc
 }
 
 // dQ of row i, without the scale
-template <typename T, int D, bool CAP, bool BIAS>
+template <typename T, int D, int CAP, bool BIAS>
 __device__ __forceinline__ void at_exact_dq(const AttArgs& a, const AtScore& sc, const AtSample& sm, int b, int head, int i, float lse, float delta, float (&dq)[2])
 {
     const int lane = threadIdx.x & 63;
@@ -123,7 +122,7 @@ __device__ __forceinline__ void at_exact_dq(const AttArgs& a, const AtScore& sc,
 }
 
 // dK (without the scale) and dV of key j over the rows `first` .. `end` - 1 of every head that reads it
-template <typename T, int D, bool CAP, bool BIAS>
+template <typename T, int D, int CAP, bool BIAS>
 __device__ __forceinline__ void at_exact_dkv(const AttArgs& a, const AtScore& sc, const AtSample& sm, const float* delta, int b, int khead, int j, int first, int end,
                                              float (&dk)[2], float (&dv)[2])
 {

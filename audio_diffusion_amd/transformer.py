@@ -5,8 +5,6 @@ They take rows ``[B, N, heads, head_dim]`` as a linear projection leaves them (v
 carry gradients.  Every call runs on the current stream of its tensors' device; outputs and workspaces come from torch's
 allocator on that stream, so a call can be captured in a graph.  No CPU or eager fallback.
 """
-import math
-
 import torch
 from torch.autograd.function import once_differentiable
 
@@ -17,6 +15,7 @@ __all__ = ["qk_norm_rope", "rope_frequencies", "masked_attention", "alibi_slopes
 _NORM_TYPES = {torch.float32: _lib.ADK_F32, torch.bfloat16: _lib.ADK_BF16, torch.float16: _lib.ADK_F16}
 _ATT_TYPES = {torch.bfloat16: _lib.ADK_BF16, torch.float16: _lib.ADK_F16}
 _pack_norm, _pack_att = _lib.packer(_lib.QkNormRopeArgs), _lib.packer(_lib.AttentionArgs)
+_LEAST = 2.0 ** -126                   # float32: below lie numbers of fewer bits, and zero
 _NO_GRADS = (0,) * 10                  # the backward fields of the norm's struct
 _NO_GRAD = (0,) * 7                    # and of the attention's
 
@@ -232,7 +231,8 @@ def masked_attention(q, k, v, *, scale=None, softcap=None, slopes=None, causal=F
     Query head h reads key head h // (Hq // Hk).  Query row i of sample b stands at position p = starts[b] + i (without
     ``starts``: Nk - Nq + i, the last rows of the keys), key j at position j.
 
-    * ``scale``: of the products, default D ** -0.5.  ``softcap`` c: scores become c tanh(score / c).
+    * ``scale``: of the products, default D ** -0.5.  ``softcap`` c: scores become c tanh(score / c), for c up to 1.1e38 (caps over 128
+      take a slower form, exact to float32 of the score however small beside the cap).
     * ``slopes`` float32 [Hq]: slopes[h] |p - j| is taken off the scores (``alibi_slopes``; constants, no gradient).
     * ``causal``: row i sees j <= p.  ``prefix`` int32 [B] (with causal): and every j < prefix[b].
     * ``lengths`` int32 [B]: keys j >= lengths[b] do not exist and are not read (values outside [0, Nk] are clamped).
@@ -255,10 +255,10 @@ def masked_attention(q, k, v, *, scale=None, softcap=None, slopes=None, causal=F
         raise ValueError(f"{what}: {Hq} query heads are not a multiple of {Hk} key heads")
     scale = D ** -0.5 if scale is None else float(scale)
     softcap = 0.0 if softcap is None else float(softcap)
-    if not (scale > 0 and math.isfinite(scale)):
-        raise ValueError(f"{what}: scale {scale} must be positive and finite")
-    if not (softcap >= 0 and math.isfinite(softcap)):
-        raise ValueError(f"{what}: softcap {softcap} must be positive and finite")
+    if not (_LEAST <= scale <= 2.3e38):
+        raise ValueError(f"{what}: scale {scale} must be in [2^-126, 2.3e38]")
+    if not (softcap == 0 or (_LEAST <= softcap <= 1.1e38 and scale <= 1.1e38 * softcap)):
+        raise ValueError(f"{what}: softcap {softcap} must be in [2^-126, 1.1e38] and at least scale / 1.1e38 (or None)")
     if not (causal or prefix is None):
         raise ValueError(f"{what}: prefix widens a causal mask: pass causal=True")
     _on_device(what, q.device, k, v, slopes, prefix, documents, lengths, starts)

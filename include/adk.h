@@ -345,7 +345,7 @@ typedef struct adk_attention_args {
     int32_t dtype;                       /* ADK_BF16 or ADK_F16                                                            */
     int32_t B, Nq, Nk, Hq, Hk, D;        /* Hq a multiple of Hk                                                            */
     int32_t causal;
-    float scale, softcap;                /* scale > 0; softcap 0: none                                                     */
+    float scale, softcap;                /* scale > 0; softcap 0: none; 1.45 scale, 2.89 softcap, 2.89 scale / softcap finite  */
     const void *q, *k, *v;               /* 16-byte aligned, strides multiples of 8 elements                               */
     int64_t q_stride_b, q_stride_n, q_stride_h, k_stride_b, k_stride_n, k_stride_h, v_stride_b, v_stride_n, v_stride_h;
     const float *slopes;                 /* f32 [Hq] or NULL                                                               */

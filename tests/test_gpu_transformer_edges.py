@@ -44,3 +44,56 @@ def test_gradients_of_keys_past_the_length_are_zeros(A, case, dt):
             within(n, x[clean], tuple(t[clean] for t in want[n]))
         for n, x, none in (("o", got[0], rows), ("dq", got[1], rows), ("dk", got[2], beyond), ("dv", got[3], beyond)):
             assert bool((x[none] == 0).all()), (n, causal)
+
+# ---- capped scores -----------------------------------------------------------------------------------------------------------
+
+CAP_CASES = {
+    "step": (3, 1, 900, 8, 2, 128, dict(lengths=True, causal=True, starts=True)),
+    "few": (2, 130, 130, 4, 1, 64, dict(causal=True, slopes=True)),
+    "few 32": (1, 190, 190, 3, 3, 32, {}),
+    "many": (4, 300, 300, 24, 8, 128, dict(causal=True)),
+    "many 64": (4, 260, 260, 32, 8, 64, dict(documents=80, causal=True)),
+    "many 32": (6, 257, 257, 32, 32, 32, dict(slopes=True)),
+    "parts": (1, 1400, 100, 4, 1, 128, {}),
+    "query parts": (1, 64, 2200, 4, 2, 64, {}),
+}
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("cap", [50.0, 128.0, 129.0, 1e3, 1e5, 1e7, 1e30, 1.1e38])
+@pytest.mark.parametrize("name", CAP_CASES)
+def test_caps_of_every_size(A, name, cap, dt):
+    """Far above the scores a cap does nothing; the error of a capped score belongs to the score, not to the cap."""
+    q, k, v, do, how = make(CAP_CASES[name], DT[dt], seed=8)
+    how["softcap"] = cap
+    want = O.attention(q, k, v, grad=do, **how)
+    for n, x in zip(("o", "dq", "dk", "dv"), graded(A, q, k, v, do, **how)):
+        within(n, x, want[n])
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("name", ["step", "few", "many", "many 64", "many 32", "parts"])
+def test_scores_of_the_caps_size_beside_small_ones(A, name, dt, monkeypatch):
+    """Cap 150; in every second row scores reach it, the rows between keep scores of order one (in the same tiles).  Beside the 1e-4 of
+    the products of scores up to 150 (see the oracle) stand 2.4e-7 times the cap from the tanh (its exponential, reciprocal
+    and difference, each off by a step of 2^-23 or half of one): 1.4e-4 together, 2e-4 allowed."""
+    monkeypatch.setattr(O, "SLACK", 2e-4)
+    q, k, v, do, how = make(CAP_CASES[name], DT[dt], seed=9)
+    q = q.clone()
+    q[:, ::2] *= 16
+    how["softcap"] = 150.0
+    how.pop("slopes", None)
+    want = O.attention(q, k, v, grad=do, **how)
+    for n, x in zip(("o", "dq", "dk", "dv"), graded(A, q, k, v, do, **how)):
+        within(n, x, want[n])
+
+
+@pytest.mark.parametrize("cap", [1e-3, 0.5])
+def test_small_caps(A, cap):
+    q, k, v, do, how = make(CAP_CASES["many 64"], torch.bfloat16, seed=10)
+    how["softcap"] = cap
+    want = O.attention(q, k, v, grad=do, **how)
+    for n, x in zip(("o", "dq", "dk", "dv"), graded(A, q, k, v, do, **how)):
+        within(n, x, want[n])
+
+

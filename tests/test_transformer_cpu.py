@@ -161,3 +161,19 @@ def test_packed_structs_have_the_mirrors_layout_and_cut_nothing_off():
             if t in (C.c_int32, C.c_float):
                 with pytest.raises(ValueError, match="beyond"):
                     pack(*values[:n], 1 << 31 if t is C.c_int32 else 1e39, *values[n + 1:])
+
+
+@pytest.mark.parametrize("kw", [dict(softcap=1.2e38), dict(softcap=3e38), dict(softcap=1e-39), dict(scale=2.4e38), dict(scale=1e30, softcap=1e-9)])
+def test_scores_outside_the_range_of_f32_are_refused(kw):
+    lib = _lib.load()
+    refused(lib.adk_attention(C.byref(att_args(**kw)), C.c_void_p(P), 1 << 40, None), "range")
+    refused(lib.adk_attention_backward(C.byref(att_args(**kw)), C.c_void_p(P), 1 << 40, None), "range")
+    for ok in (dict(softcap=1.1e38), dict(softcap=1e-30), dict(scale=2.3e38), dict(scale=1e-30)):
+        assert lib.adk_attention_workspace(C.byref(att_args(**ok)), 0) >= 0
+
+
+@pytest.mark.parametrize("kw", [dict(softcap=1e-50), dict(softcap=1e-46), dict(scale=1e-50)])
+def test_a_cap_or_scale_that_f32_does_not_have_is_refused(kw):
+    """and is not taken for no cap."""
+    with pytest.raises(ValueError, match=next(iter(kw))):
+        A.masked_attention(*qkv(), **kw)
