@@ -5,5 +5,7 @@ int att_backward_bf16(const AttArgs& a, void* ws, hipStream_t st) { return att_b
 
 long long att_backward_workspace(const AttArgs& a)
 {
-    return att_doc_bytes(a) + att_round((long long)a.B * a.Hq * a.Nq * 4) * (a.dtype == ADK_F16 ? 2 : 1) + att_round((long long)a.B * a.Hq * att_bwd_qtiles(a) * 4) + att_bwd_part(a);
+    const long long rows = att_round((long long)a.B * a.Hq * a.Nq * 4);
+    const long long f16 = 2 * rows + att_round((long long)a.B * a.Hq * att_bwd_groups(a) * 4) + att_round((long long)a.B * a.Hk * a.Nk * 4);
+    return att_doc_bytes(a) + rows + (a.dtype == ADK_F16 ? f16 : 0) + att_bwd_part(a);
 }

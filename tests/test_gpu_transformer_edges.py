@@ -97,3 +97,50 @@ def test_small_caps(A, cap):
         within(n, x, want[n])
 
 
+
+# ---- f16's range -------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("D, Hq, Hk", [(32, 2, 1), (64, 4, 2), (128, 4, 1)])
+def test_f16_gradients_of_keys_of_a_quiet_document(A, D, Hq, Hk):
+    """Two documents whose gradients are 2^14 apart: the quiet one's are as exact as on their own."""
+    N, half = 3000, 1500
+    q, k, v, do, _ = make((1, N, N, Hq, Hk, D, {}), torch.float16, seed=11)
+    docs = (torch.arange(N, device="cuda") >= half).int()[None]
+    mix = (torch.arange(N, device="cuda") % 3 == 1).int()[None]                # taking turns: both in every tile
+    for d in (docs, mix):
+        g = torch.where(d[..., None, None] == 0, do * 2.0 ** 10, do * 2.0 ** -4)
+        got = graded(A, q, k, v, g, documents=d)
+        for which in (0, 1):
+            at = d[0] == which
+            want = O.attention(*(t[:, at] for t in (q, k, v)), grad=g[:, at])
+            for n, x in zip(("o", "dq", "dk", "dv"), got):
+                within(f"{n} of document {which}", x[:, at], want[n])
+
+
+@pytest.mark.parametrize("D", [32, 64, 128])
+def test_f16_gradients_of_keys_that_only_quiet_rows_see(A, D):
+    """Causal: the last rows' gradients are 2^14 smaller than the first ones', and the last keys are seen by those alone."""
+    N, half = 1100, 700
+    q, k, v, do, _ = make((1, N, N, 4, 2, D, {}), torch.float16, seed=12)
+    quiet = (torch.arange(N, device="cuda") >= half)[None, :, None, None]
+    g = torch.where(quiet, do * 2.0 ** -4, do * 2.0 ** 10)
+    got = graded(A, q, k, v, g, causal=True)
+    want = O.attention(q, k, v, grad=g, causal=True)
+    for n, x in zip(("o", "dq", "dk", "dv"), got):
+        within(n, x, want[n])
+    alone = O.attention(q, k, v, grad=torch.where(quiet, g, 0.0), causal=True)
+    for n, x in zip(("dk", "dv"), got[2:]):
+        within(f"{n} of the last keys", x[:, half:], tuple(t[:, half:] for t in alone[n]))
+
+
+@pytest.mark.parametrize("scale", [2.0 ** -10, 1.0, 1000.0])
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("case", [(2, 260, 260, 8, 2, 64), (2, 300, 300, 4, 1, 128)], ids=lambda c: "-".join(map(str, c)))
+def test_gradients_of_other_sizes(A, case, dt, scale):
+    q, k, v, do, how = make(case + (dict(causal=True, documents=90),), DT[dt], seed=13)
+    do = do * scale
+    want = O.attention(q, k, v, grad=do, **how)
+    for n, x in zip(("o", "dq", "dk", "dv"), graded(A, q, k, v, do, **how)):
+        within(n, x, want[n])
+
+
