@@ -168,6 +168,12 @@ template <int CAP> __device__ __forceinline__ float at_capped(float qk, const At
     return at_score<CAP>(sc, qk, 0.f, th);
 }
 
+// The running maximum of the forward kernels is kept this much lower, so that a probability is at most 2^(8 + this) before it is rounded (8: see
+// masked_attention_fwd.inc).  f16 ends at 2^16 and has its smallest step at 2^-24: taken relative to the maximum itself, the keys of a long row that
+// hold 2^-25 each are counted in the sum and lost in the product (65536 of them: 0.2 % of the row).  bf16 has f32's range.
+template <typename T> __device__ __forceinline__ constexpr float at_raised() { return 0.f; }
+template <> __device__ __forceinline__ constexpr float at_raised<f16_t>() { return 7.f; }
+
 // ---- LDS tiles -----------------------------------------------------------------------------------------------------------
 // A tile is [rows][D] 16-bit, rows of 2 D bytes, filled by LDS-DMA (1 KiB per wave instruction, lane l at + 16 l).  Piece p
 // (16 bytes) of row r sits in slot p ^ swz(r): reading one piece of 8 consecutive rows (row fragments) and 4 pieces of

@@ -1,5 +1,7 @@
 """Token-sequence operators on the GPU at their edges, against the same 64-bit statements (oracle/token_ops_oracle.py).  Tolerances are
 that file's unless a test derives its own."""
+import math
+
 import pytest
 import torch
 
@@ -144,3 +146,19 @@ def test_gradients_of_other_sizes(A, case, dt, scale):
         within(n, x, want[n])
 
 
+
+@pytest.mark.parametrize("case", [(1, 1, 1 << 17, 2, 1, 64), (1, 2048, 1 << 16, 4, 1, 64), (1, 2048, 1 << 16, 12, 1, 128)], ids=lambda c: "-".join(map(str, c)))
+def test_f16_many_small_probabilities(A, case):
+    """One key holds nearly all, the others 2^-25 of it each, and only they have values.  A probability is rounded to f16's step of 2^-24
+    at most after it was taken relative to 2^-7 of the largest: 2^-32 is the largest error of each, not 2^-25."""
+    B, Nq, Nk, Hq, Hk, D = case
+    q = torch.zeros(B, Nq, Hq, D, dtype=torch.float16, device="cuda")
+    k = torch.zeros(B, Nk, Hk, D, dtype=torch.float16, device="cuda")
+    v = torch.ones(B, Nk, Hk, D, dtype=torch.float16, device="cuda")
+    q[..., 0] = 1.0
+    k[:, Nk // 3, :, 0] = 25.0
+    v[:, Nk // 3] = 0.0
+    o = A.masked_attention(q, k, v, scale=math.log(2.0)).double()
+    rest = (Nk - 1) * 2.0 ** -25
+    want = rest / (1 + rest)
+    assert float((o - want).abs().max()) <= (1e-4 + 2.0 ** -10) * want + Nk * 2.0 ** -32, (float(o.min()), float(o.max()), want)
