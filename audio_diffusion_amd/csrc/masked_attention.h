@@ -63,13 +63,13 @@ __device__ __forceinline__ int at_limit(const AttArgs& a, const AtSample& s, int
     return a.causal ? min(s.klen - 1, max(s.start + i, s.prefix - 1)) : s.klen - 1;
 }
 // The position a distance is taken from: outside the keys the distances differ from those of the nearest end by a constant
-// of the row, which the softmax does not see.
-__device__ __forceinline__ float at_bias_pos(const AttArgs& a, const AtSample& s, int i) { return (float)min(max(s.start + i, 0), a.Nk - 1); }
+// of the row, which the softmax does not see.  Whole numbers: their difference is rounded to f32, not they (behind key 2^24 f32 skips keys).
+__device__ __forceinline__ int at_bias_pos(const AttArgs& a, const AtSample& s, int i) { return min(max(s.start + i, 0), a.Nk - 1); }
 // The bias -slope |pos - j| of a tile of 64 keys from k0 is side * (j - pos) where all keys stand on one side of the positions first .. last
 // (0: they do not, or there is no bias).
-__device__ __forceinline__ float at_side(float slope, int k0, float first, float last)
+__device__ __forceinline__ float at_side(float slope, int k0, int first, int last)
 {
-    return (float)(k0 + AT_KT - 1) <= first ? slope : (float)k0 >= last ? -slope : 0.f;
+    return k0 + AT_KT - 1 <= first ? slope : k0 >= last ? -slope : 0.f;
 }
 __device__ __forceinline__ int at_row_doc(const AttArgs& a, const AtSample& s, int b, int i)       // negative: none
 {

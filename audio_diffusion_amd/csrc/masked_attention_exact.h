@@ -69,13 +69,14 @@ __device__ __forceinline__ void at_exact_row(const AttArgs& a, const AtScore& sc
     const AtOperands<T> p = at_operands<T>(a, b, head);
     const T* qr = p.q + (long long)i * a.q_stride_n;
     const int doc = a.documents ? at_row_doc(a, sm, b, i) : 0, lim = doc < 0 ? -1 : min(at_limit(a, sm, i), j1 - 1);
-    const float pos = at_bias_pos(a, sm, i), slope2 = BIAS ? a.slopes[head] * AT_LOG2E : 0.f;
+    const int pos = at_bias_pos(a, sm, i);
+    const float slope2 = BIAS ? a.slopes[head] * AT_LOG2E : 0.f;
     m = -INFINITY; l = 0.f; o[0] = o[1] = 0.f;
     for (int jb = j0; jb <= lim; jb += 64) {
         const int j = jb + lane;
         const bool see = j <= lim && (!a.documents || a.documents[(long long)b * a.documents_stride + j] == doc);
         float x = -INFINITY, th;
-        if (see) x = at_base2<CAP, BIAS>(sc, at_dot<T, D>(qr, p.k + (long long)j * a.k_stride_n), slope2, pos - (float)j, th);
+        if (see) x = at_base2<CAP, BIAS>(sc, at_dot<T, D>(qr, p.k + (long long)j * a.k_stride_n), slope2, (float)(pos - j), th);
         unsigned long long seen = __ballot(see);
         if (!seen) continue;
         const float mn = __builtin_elementwise_maximum(m, at_wave_max(x)), f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
@@ -101,14 +102,15 @@ __device__ __forceinline__ void at_exact_dq(const AttArgs& a, const AtScore& sc,
     const AtOperands<T> p = at_operands<T>(a, b, head);
     const T *qr = p.q + (long long)i * a.q_stride_n, *gr = p.g + (long long)i * a.og_stride_n;
     const int doc = a.documents ? at_row_doc(a, sm, b, i) : 0, lim = doc < 0 ? -1 : at_limit(a, sm, i);
-    const float pos = at_bias_pos(a, sm, i), slope2 = BIAS ? a.slopes[head] * AT_LOG2E : 0.f;
+    const int pos = at_bias_pos(a, sm, i);
+    const float slope2 = BIAS ? a.slopes[head] * AT_LOG2E : 0.f;
     dq[0] = dq[1] = 0.f;
     for (int jb = 0; jb <= lim; jb += 64) {
         const int j = jb + lane;
         const bool see = j <= lim && (!a.documents || a.documents[(long long)b * a.documents_stride + j] == doc);
         float ds = 0.f, th;
         if (see) {
-            const float x = at_base2<CAP, BIAS>(sc, at_dot<T, D>(qr, p.k + (long long)j * a.k_stride_n), slope2, pos - (float)j, th);
+            const float x = at_base2<CAP, BIAS>(sc, at_dot<T, D>(qr, p.k + (long long)j * a.k_stride_n), slope2, (float)(pos - j), th);
             ds = __builtin_amdgcn_exp2f(x - lse) * (at_dot<T, D>(gr, p.v + (long long)j * a.v_stride_n) - delta) * (1.f - th * th);
         }
         for (unsigned long long seen = __ballot(see); seen; seen &= seen - 1) {
@@ -141,7 +143,7 @@ __device__ __forceinline__ void at_exact_dkv(const AttArgs& a, const AtScore& sc
             const bool see = i < end && (!a.documents || at_row_doc(a, sm, b, i) == doc);
             float ds = 0.f, pr = 0.f, th;
             if (see) {
-                const float x = at_base2<CAP, BIAS>(sc, at_dot<T, D>(p.q + (long long)i * a.q_stride_n, kr), slope2, at_bias_pos(a, sm, i) - (float)j, th);
+                const float x = at_base2<CAP, BIAS>(sc, at_dot<T, D>(p.q + (long long)i * a.q_stride_n, kr), slope2, (float)(at_bias_pos(a, sm, i) - j), th);
                 pr = __builtin_amdgcn_exp2f(x - a.lse[at + i]);
                 ds = pr * (at_dot<T, D>(p.g + (long long)i * a.og_stride_n, vr) - delta[at + i]) * (1.f - th * th);
             }

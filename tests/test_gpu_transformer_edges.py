@@ -162,3 +162,25 @@ def test_f16_many_small_probabilities(A, case):
     rest = (Nk - 1) * 2.0 ** -25
     want = rest / (1 + rest)
     assert float((o - want).abs().max()) <= (1e-4 + 2.0 ** -10) * want + Nk * 2.0 ** -32, (float(o.min()), float(o.max()), want)
+
+
+# ---- far keys ----------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("Nq, Hq", [(1, 2), (130, 2), (2048, 16)])
+def test_distances_behind_2_to_the_24th_key(A, Nq, Hq):
+    """Distances of a bias are whole numbers up to rounding of the DISTANCE, wherever the keys stand."""
+    Nk, D, tail = (1 << 24) + 4099, 32, 2048 + 512
+    g = gen(14)
+    q, do = randn(g, 1, Nq, Hq, D, dtype=torch.bfloat16), randn(g, 1, Nq, Hq, D, dtype=torch.bfloat16)
+    kt, vt = randn(g, 1, tail, 1, D, dtype=torch.bfloat16), randn(g, 1, tail, 1, D, dtype=torch.bfloat16)
+    k = torch.zeros(1, Nk, 1, D, dtype=torch.bfloat16, device="cuda")
+    v = torch.zeros(1, Nk, 1, D, dtype=torch.bfloat16, device="cuda")
+    k[:, Nk - tail:], v[:, Nk - tail:] = kt, vt
+    docs = torch.full((1, Nk), -1, dtype=torch.int32, device="cuda")
+    docs[:, Nk - tail:] = 3
+    slopes = torch.linspace(0.3, 1.5, Hq, device="cuda")
+    for causal in (True, False):
+        want = O.attention(q, kt, vt, grad=do, slopes=slopes, causal=causal)       # the tail alone
+        got = graded(A, q, k, v, do, slopes=slopes, causal=causal, documents=docs)
+        for n, x in zip(("o", "dq", "dk", "dv"), got):
+            within(n, x[:, Nk - tail:] if n in ("dk", "dv") else x, want[n])
