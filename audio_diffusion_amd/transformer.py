@@ -6,6 +6,7 @@ carry gradients.  Every call runs on the current stream of its tensors' device; 
 allocator on that stream, so a call can be captured in a graph.  No CPU or eager fallback.
 """
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -49,6 +50,16 @@ def _on_device(what, device, *tensors):
     for t in tensors:
         if t is not None and t.get_device() != index:          # -1 on the CPU
             raise ValueError(f"{what}: tensors on {t.device} and {device}")
+
+
+def _no_recording(what, *tensors):
+    """The library writes through pointers: a forward-mode tangent, or a trace, would be dropped without a word."""
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError(f"{what}: forward-mode derivatives are not built")
+    if torch._C._get_tracing_state() is not None:
+        raise NotImplementedError(f"{what}: cannot be recorded by torch.jit.trace")
 
 
 def _rows(t):
@@ -112,6 +123,7 @@ class _QkNormRope(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, gq, gk):
+        _no_recording("qk_norm_rope backward", gq, gk)
         q, k, q_weight, k_weight, positions, frequencies = ctx.saved_tensors
         gq, gk = _rows(gq), _rows(gk)
         dq, dk = _like(q), _like(k)
@@ -136,7 +148,7 @@ def qk_norm_rope(q, k, q_weight, k_weight, positions, frequencies, eps=1e-6, int
     * ``positions``: int32 or int64, [N] or [B, N], any values (expanded views are read as they are).
     * ``frequencies``: float64 [R / 2], radians per position (``rope_frequencies``); may be empty (norm only).
     * ``interleaved``: pairs (2p, 2p + 1) instead of (p, p + R / 2).
-    Gradients flow to q, k and the weights, not to positions or frequencies.
+    Gradients (reverse mode, once) flow to q, k and the weights, not to positions or frequencies.
     """
     what = "qk_norm_rope"
     if not (q.dim() == 4 and k.dim() == 4 and q.shape[:2] == k.shape[:2] and q.shape[3] == k.shape[3]):
@@ -163,6 +175,7 @@ def qk_norm_rope(q, k, q_weight, k_weight, positions, frequencies, eps=1e-6, int
             raise ValueError(f"{what}: a weight is not a floating [{D}]")
     if frequencies.requires_grad:
         raise ValueError(f"{what}: no gradient to frequencies is built")
+    _no_recording(what, q, k, q_weight, k_weight, frequencies)
     _on_device(what, q.device, k, q_weight, k_weight, positions, frequencies)
     if positions.dim() == 1:
         positions = positions.expand(B, N)
@@ -205,6 +218,7 @@ class _MaskedAttention(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, go):
+        _no_recording("masked_attention backward", go)
         q, k, v, slopes, prefix, documents, lengths, starts, o, lse = ctx.saved_tensors
         dq, dk, dv = _like(q), _like(k), _like(v)
         if q.numel() == 0:
@@ -239,8 +253,8 @@ def masked_attention(q, k, v, *, scale=None, softcap=None, slopes=None, causal=F
     * ``documents`` int32 [B, Nk]: row i sees keys of its own document, documents[b, p]; negative ids are padding, and
       rows at a position outside [0, Nk) have no document.
     A row that sees nothing gives zeros.  bfloat16 and float16, D = 32, 64 or 128, any strides (rows whose heads are not 16-byte
-    aligned are copied first).  Gradients flow to q, k and v, with a fixed summation order.  A single new token over a long
-    cache (Nq = 1) is split over the keys.
+    aligned are copied first).  Gradients (reverse mode, once) flow to q, k and v, with a fixed summation order.  A single new
+    token over a long cache (Nq = 1) is split over the keys.
     """
     what = "masked_attention"
     if not (q.dim() == 4 and k.dim() == 4 and k.shape == v.shape and q.shape[0] == k.shape[0] and q.shape[3] == k.shape[3]):
@@ -261,6 +275,7 @@ def masked_attention(q, k, v, *, scale=None, softcap=None, slopes=None, causal=F
         raise ValueError(f"{what}: softcap {softcap} must be in [2^-126, 1.1e38] and at least scale / 1.1e38 (or None)")
     if not (causal or prefix is None):
         raise ValueError(f"{what}: prefix widens a causal mask: pass causal=True")
+    _no_recording(what, q, k, v, slopes)
     _on_device(what, q.device, k, v, slopes, prefix, documents, lengths, starts)
     if slopes is not None:
         if not (slopes.dtype == torch.float32 and tuple(slopes.shape) == (Hq,)):

@@ -184,3 +184,18 @@ def test_distances_behind_2_to_the_24th_key(A, Nq, Hq):
         got = graded(A, q, k, v, do, slopes=slopes, causal=causal, documents=docs)
         for n, x in zip(("o", "dq", "dk", "dv"), got):
             within(n, x[:, Nk - tail:] if n in ("dk", "dv") else x, want[n])
+
+
+# ---- what is not built --------------------------------------------------------------------------------------------------------
+
+def test_tangents_of_gradients_are_refused(A):
+    q, k, v, do, _ = make((1, 20, 20, 2, 1, 64, {}), torch.bfloat16)
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    f, pos = A.rope_frequencies(64, device="cuda"), torch.arange(20, device="cuda")
+    o, y = A.masked_attention(*leaves), A.qk_norm_rope(leaves[0], leaves[1], None, None, pos, f)[0]
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(do, torch.ones_like(do))
+        for out in (o, y):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                torch.autograd.grad(out, leaves[0], dual, retain_graph=True)
+        assert all(bool(torch.isfinite(g).all()) for g in torch.autograd.grad(o, leaves, do))      # a plain gradient passes

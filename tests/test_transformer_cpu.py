@@ -177,3 +177,26 @@ def test_a_cap_or_scale_that_f32_does_not_have_is_refused(kw):
     """and is not taken for no cap."""
     with pytest.raises(ValueError, match=next(iter(kw))):
         A.masked_attention(*qkv(), **kw)
+
+
+def test_forward_mode_tangents_and_traces_are_refused_not_dropped():
+    """(Before the tensors' device is looked at.)  Plain tensors inside a dual level pass on to the next check."""
+    q, k, v = qkv(Nk=3)
+    pos, f, w, s = torch.arange(3), A.rope_frequencies(64), torch.ones(64), torch.ones(4)
+    with torch.autograd.forward_ad.dual_level():
+        dual = lambda t: torch.autograd.forward_ad.make_dual(t, torch.ones_like(t))          # noqa: E731
+        for args in ((dual(q), k, v), (q, dual(k), v), (q, k, dual(v))):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                A.masked_attention(*args)
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            A.masked_attention(q, k, v, slopes=dual(s))
+        for args in ((dual(q), k, w, w, pos, f), (q, dual(k), w, w, pos, f), (q, k, dual(w), w, pos, f), (q, k, w, dual(w), pos, f), (q, k, w, w, pos, dual(f))):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                A.qk_norm_rope(*args)
+        with pytest.raises(RuntimeError, match="no CPU path"):
+            A.masked_attention(q, k, v)
+        with pytest.raises(RuntimeError, match="no CPU path"):
+            A.qk_norm_rope(q, k, w, w, pos, f)
+    for fn, args in ((A.masked_attention, (q, k, v)), (lambda q, k: A.qk_norm_rope(q, k, w, w, pos, f), (q, k))):
+        with pytest.raises(NotImplementedError, match="trace"):
+            torch.jit.trace(fn, args)
