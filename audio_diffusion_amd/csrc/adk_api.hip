@@ -617,16 +617,19 @@ static int check_att(const AttArgs* a, bool grad, const char* what)
     if (a->B == 0 || a->Nq == 0) return ADK_OK;            // no rows
     REQUIRE(a->q && a->o && (a->Nk == 0 || (a->k && a->v)), "%s: null tensor", what);
     auto al = [](const void* p) { return ((uintptr_t)p & 15) == 0; };
-    auto s8 = [](int64_t x, int64_t y, int64_t z) { return x % 8 == 0 && y % 8 == 0 && z % 8 == 0; };
-    REQUIRE(al(a->q) && al(a->k) && al(a->v) && al(a->o), "%s: q, k, v and o must be 16-byte aligned", what);
-    REQUIRE(s8(a->q_stride_b, a->q_stride_n, a->q_stride_h) && s8(a->k_stride_b, a->k_stride_n, a->k_stride_h)
-            && s8(a->v_stride_b, a->v_stride_n, a->v_stride_h), "%s: strides must be multiples of 8 elements", what);
-    auto row = [](int64_t s) { return s >= 0 && s <= (1 << 24); };
-    REQUIRE(row(a->q_stride_n) && row(a->k_stride_n) && row(a->v_stride_n) && (!grad || row(a->og_stride_n)),
+    // the stride of a dimension of one is not used; nor are any of a tensor without elements
+    auto s8 = [&](int N, int H, int64_t b, int64_t n, int64_t h) {
+        return N == 0 || ((a->B == 1 || b % 8 == 0) && (N == 1 || n % 8 == 0) && (H == 1 || h % 8 == 0));
+    };
+    auto row = [](int N, int64_t s) { return N <= 1 || (s >= 0 && s <= (1 << 24)); };
+    REQUIRE(al(a->q) && al(a->o) && (a->Nk == 0 || (al(a->k) && al(a->v))), "%s: q, k, v and o must be 16-byte aligned", what);
+    REQUIRE(s8(a->Nq, a->Hq, a->q_stride_b, a->q_stride_n, a->q_stride_h) && s8(a->Nk, a->Hk, a->k_stride_b, a->k_stride_n, a->k_stride_h)
+            && s8(a->Nk, a->Hk, a->v_stride_b, a->v_stride_n, a->v_stride_h), "%s: strides must be multiples of 8 elements", what);
+    REQUIRE(row(a->Nq, a->q_stride_n) && row(a->Nk, a->k_stride_n) && row(a->Nk, a->v_stride_n) && (!grad || row(a->Nq, a->og_stride_n)),
             "%s: a row stride is not in [0, 2^24] elements", what);
     if (grad) {
         REQUIRE(a->lse && a->o_grad && a->q_grad && (a->Nk == 0 || (a->k_grad && a->v_grad)), "%s: null tensor", what);
-        REQUIRE(al(a->o_grad) && al(a->q_grad) && al(a->k_grad) && al(a->v_grad) && s8(a->og_stride_b, a->og_stride_n, a->og_stride_h),
+        REQUIRE(al(a->o_grad) && al(a->q_grad) && (a->Nk == 0 || (al(a->k_grad) && al(a->v_grad))) && s8(a->Nq, a->Hq, a->og_stride_b, a->og_stride_n, a->og_stride_h),
                 "%s: gradients must be 16-byte aligned with strides of multiples of 8 elements", what);
     }
     return ADK_OK;

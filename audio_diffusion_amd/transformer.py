@@ -68,9 +68,13 @@ def _rows(t):
 
 
 def _rows16(t):
-    """Rows with 16-byte aligned heads, at most 2^24 elements apart (a copy if they are not)."""
+    """Rows with 16-byte aligned heads, at most 2^24 elements apart (a copy if they are not).  The stride of a dimension of one, which a
+    slice may leave at anything, does not matter (nor does it to the library, and contiguous() leaves it as it is)."""
     sb, sn, sh, sd = t.stride()
     if sd == 1 and not ((sb | sn | sh) & 7) and sn <= 1 << 24 and not (t.data_ptr() & 15):
+        return t
+    B, N, H, _ = t.shape
+    if sd == 1 and not ((sb * (B > 1) | sn * (N > 1) | sh * (H > 1)) & 7) and (sn <= 1 << 24 or N == 1) and not (t.data_ptr() & 15):
         return t
     t = t.contiguous()
     return t if not (t.data_ptr() & 15) else t.clone()

@@ -340,7 +340,8 @@ int adk_qk_norm_rope_backward(const adk_qk_norm_rope_args *args, void *workspace
  *   o = softmax over the seen keys, times v.  A row that sees no key gives zeros (and no gradient).
  * Query head h reads key head h / (Hq / Hk).  16-bit types; D = 32, 64 or 128; products of 16-bit values are summed in f32,
  * probabilities are rounded to the type for the second product, and in the backward dS for its products.  Keys at and past
- * lengths[b] are not read; starts, lengths and prefix may hold any int32.  Row strides (*_stride_n) lie in [0, 2^24]. */
+ * lengths[b] are not read; starts, lengths and prefix may hold any int32.  Row strides (*_stride_n) lie in [0, 2^24].  The stride of a
+ * dimension of one may be anything. */
 typedef struct adk_attention_args {
     int32_t dtype;                       /* ADK_BF16 or ADK_F16                                                            */
     int32_t B, Nq, Nk, Hq, Hk, D;        /* Hq a multiple of Hk                                                            */

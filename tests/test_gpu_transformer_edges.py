@@ -199,3 +199,32 @@ def test_tangents_of_gradients_are_refused(A):
             with pytest.raises(NotImplementedError, match="forward-mode"):
                 torch.autograd.grad(out, leaves[0], dual, retain_graph=True)
         assert all(bool(torch.isfinite(g).all()) for g in torch.autograd.grad(o, leaves, do))      # a plain gradient passes
+
+
+# ---- views ---------------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("shape", [(1, 150, 150, 4, 2), (1, 1, 900, 8, 2), (2, 1, 1, 4, 1), (1, 40, 40, 1, 1), (3, 1, 70, 1, 1), (1, 300, 1, 2, 1)], ids=lambda c: "-".join(map(str, c)))
+def test_views_with_odd_strides_of_dimensions_of_one(A, shape):
+    """One sample of a padded buffer, one token, one head: the same bits as contiguous tensors; the incoming gradient too."""
+    B, Nq, Nk, Hq, Hk = shape
+    q, k, v, do, _ = make((B, Nq, Nk, Hq, Hk, 64, {}), torch.bfloat16, seed=16)
+
+    def odd(t):
+        """t with the strides of its dimensions of one set to 67."""
+        return t.as_strided(t.shape, [67 if n == 1 else s for n, s in zip(t.shape, t.stride())])
+
+    assert any(s == 67 for t in (q, k, do) for s in odd(t).stride())
+    base = graded(A, q, k, v, do, causal=True)
+    leaves = [odd(t).detach().requires_grad_() for t in (q, k, v)]
+    o = A.masked_attention(*leaves, causal=True)
+    for x, y in zip(base, (o,) + torch.autograd.grad(o, leaves, odd(do))):
+        assert torch.equal(x, y)
+    for x, y in zip(base, graded(A, *(odd(t) for t in (q, k, v, do)), causal=True)):
+        assert torch.equal(x, y)
+
+
+def test_an_empty_cache_with_odd_strides(A):
+    q = torch.ones(2, 3, 2, 64, dtype=torch.float16, device="cuda")
+    k = torch.ones(2, 5, 2, 67, dtype=torch.float16, device="cuda")[:, :0, :, 1:65]
+    got = graded(A, q, k, k, q, causal=True)
+    assert got[2].shape == (2, 0, 2, 64) and not any(bool(t.any()) for t in got)

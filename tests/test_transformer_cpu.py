@@ -200,3 +200,26 @@ def test_forward_mode_tangents_and_traces_are_refused_not_dropped():
     for fn, args in ((A.masked_attention, (q, k, v)), (lambda q, k: A.qk_norm_rope(q, k, w, w, pos, f), (q, k))):
         with pytest.raises(NotImplementedError, match="trace"):
             torch.jit.trace(fn, args)
+
+
+def test_strides_of_dimensions_of_one_do_not_matter():
+    """Views that torch calls contiguous whatever the stride of a dimension of one: nothing is copied, nothing refused."""
+    from audio_diffusion_amd import transformer as T
+    bf = torch.bfloat16
+    for t in (torch.zeros(2, 643, dtype=bf)[:, :640].view(2, 5, 2, 64)[:1],                  # one sample of a padded buffer
+              torch.zeros(1, 6, 1, 67, dtype=bf)[:, :1, :, :64],                              # one token of one padded head
+              torch.zeros(2, 3, 67, 64, dtype=bf).transpose(1, 2)[:, :, 1:2][:1, :1],
+              torch.zeros(1, 1, 1, (1 << 24) + 64, dtype=bf)[..., :64].expand(3, 1, 1, 64)):
+        assert T._rows16(t) is t, t.stride()
+        assert t.shape[-1] == 64
+    odd = torch.zeros(2, 643, dtype=bf)[:, :640].view(2, 5, 2, 64)                            # two samples: copied
+    assert T._rows16(odd) is not odd and T._rows16(odd).stride() == (640, 128, 64, 1)
+    lib = _lib.load()
+    docs = dict(documents=P, documents_stride=40)                                             # a call that needs a workspace: refused for that alone
+    for kw in (dict(B=1, q_stride_b=643, k_stride_b=3, v_stride_b=-5, og_stride_b=1), dict(Nq=1, q_stride_n=67, og_stride_n=-3), dict(Nq=1, q_stride_n=1 << 30),
+               dict(Hq=1, Hk=1, q_stride_h=67, k_stride_h=67, v_stride_h=1, og_stride_h=9), dict(Nk=1, k_stride_n=67, v_stride_n=1 << 40),
+               dict(Nk=0, k=P + 2, v=P + 2, k_stride_b=3, v_stride_h=5, k_stride_n=-7)):
+        if kw.get("Nk") != 0:                                                                 # (no keys: no ranges of documents)
+            refused(lib.adk_attention(C.byref(att_args(**docs, **kw)), None, 0, None), "workspace")
+        refused(lib.adk_attention_backward(C.byref(att_args(**docs, **kw)), None, 0, None), "workspace")
+        refused(lib.adk_attention_backward(C.byref(att_args(**docs, **dict(kw, Nq=2, B=2, Hq=2, Hk=2, Nk=2, k=P, v=P))), None, 0, None), "stride")
