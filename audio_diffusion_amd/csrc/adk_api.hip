@@ -608,7 +608,8 @@ static int check_att(const AttArgs* a, bool grad, const char* what)
     REQUIRE(a->B >= 0 && a->Nq >= 0 && a->Nk >= 0 && a->Nq <= (1 << 28) && a->Nk <= (1 << 28), "%s: B=%d Nq=%d Nk=%d (lengths up to 2^28)",
             what, a->B, a->Nq, a->Nk);
     REQUIRE(a->B <= 65535 && (long long)a->B * a->Hq * ((a->Nq + 31LL) / 32) < (1LL << 30) && (long long)a->B * a->Hk * ((a->Nk + 31LL) / 32) < (1LL << 30)
-            && (long long)a->Nq * (a->Hq / a->Hk) < (1LL << 30), "%s: B=%d x heads %d / %d x rows %d / %d exceed the grid", what, a->B, a->Hq, a->Hk, a->Nq, a->Nk);
+            && (long long)a->Nq * (a->Hq / a->Hk) < (1LL << 30) && att_grids_fit(*a, grad), "%s: B=%d x heads %d / %d x rows %d / %d exceed the grid", what,
+            a->B, a->Hq, a->Hk, a->Nq, a->Nk);
     REQUIRE(a->scale > 0.f && a->scale <= 3.0e38f, "%s: scale=%g must be positive and finite", what, (double)a->scale);
     REQUIRE(a->softcap >= 0.f && a->softcap <= 3.0e38f, "%s: softcap=%g must be positive and finite, or 0", what, (double)a->softcap);
     REQUIRE(at_scores_finite(*a), "%s: scale=%g, softcap=%g: 1.45 scale, 2.89 scale / softcap and 2.89 softcap must be within the range of f32", what,

@@ -371,7 +371,7 @@ __device__ __forceinline__ AtWalk<NW> at_walk(const AttArgs& a, const int* all_r
 // (4096 rows) 83 / 64.
 // Its own blocks are split over the keys to fill the card once, at least 512 keys each (below that the joining costs more than it gains:
 // 4096 keys, 8 key heads of 128: 13.8 us, split to 256 keys 15.6) and, so that caches of unequal fill come out even, at most about 4096 (8 caches of 32 to
-// 64 Ki keys: 304 us, four splits of each 323).
+// 64 Ki keys: 304 us, four splits of each 323); 2^16 blocks are even enough for any cache, and bound the partial sums.
 struct AtStepPlan { bool use; int nsplit; };
 static inline AtStepPlan at_step_plan(const AttArgs& a)
 {
@@ -383,9 +383,17 @@ static inline AtStepPlan at_step_plan(const AttArgs& a)
         const long long fill = 256 / items, even = items < 2048 ? a.Nk / 4096 : 0, most = a.Nk / 512;
         long long n = fill > even ? fill : even;
         n = n < most ? n : most;
+        n = n < 65536 / items ? n : 65536 / items;
         p.nsplit = n < 1 ? 1 : (int)n;
     }
     return p;
+}
+// A launch has fewer than 2^32 threads.  (The backward kernels are split, at most 2048 blocks of them, only where their blocks are few.)
+static inline bool att_grids_fit(const AttArgs& a, bool grad)
+{
+    const long long rows = (long long)a.B * a.Hq * ((a.Nq + 255LL) / 256) * 512, G = a.Hq / a.Hk, most = 1LL << 32;
+    if (grad) return rows < most && (long long)a.B * a.Hk * ((a.Nk + 127LL) / 128) * 256 < most;
+    return at_step_plan(a).use ? (long long)a.B * a.Hk * ((a.Nq * G + 31) / 32) * 256 < most : rows < most;
 }
 
 // ---- launchers (one translation unit per type) -----------------------------------------------------------------------------

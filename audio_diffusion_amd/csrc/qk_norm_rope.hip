@@ -205,7 +205,7 @@ __global__ __launch_bounds__(64 * QK_WAVES) void qk_fwd_kernel(const QkArgs a, c
     typedef QkRow<T, VEC> Row;
     __shared__ float2 cs_all[QK_WAVES][QK_MAX_PAIRS];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const long long item = (long long)blockIdx.x * QK_WAVES + wave;
+    const long long item = ((long long)blockIdx.y * gridDim.x + blockIdx.x) * QK_WAVES + wave;
     if (item >= gr.tokens * gr.chunks) return;                     // wave-uniform; no block barrier in this kernel
     const long long token = item / gr.chunks;
     const int ch = (int)(item % gr.chunks), b = (int)(token / a.N), n = (int)(token % a.N);
@@ -396,7 +396,9 @@ template <typename T> static int launch_qk_t(const QkArgs& a, void* ws, hipStrea
             g.chunks = (H + g.chunk - 1) / g.chunk;
         }
         const long long items = g.tokens * g.chunks;
-        const dim3 grid((unsigned)((items + QK_WAVES - 1) / QK_WAVES));
+        // (a row of the grid has fewer than 2^32 threads)
+        const long long blocks = (items + QK_WAVES - 1) / QK_WAVES, row = 1LL << 22;
+        const dim3 grid((unsigned)(blocks < row ? blocks : row), (unsigned)((blocks + row - 1) / row));
         if (vec) {
             if (a.interleaved) hipLaunchKernelGGL((qk_fwd_kernel<T, true, true>), grid, dim3(64 * QK_WAVES), 0, st, a, g);
             else hipLaunchKernelGGL((qk_fwd_kernel<T, true, false>), grid, dim3(64 * QK_WAVES), 0, st, a, g);

@@ -228,3 +228,20 @@ def test_an_empty_cache_with_odd_strides(A):
     k = torch.ones(2, 5, 2, 67, dtype=torch.float16, device="cuda")[:, :0, :, 1:65]
     got = graded(A, q, k, k, q, causal=True)
     assert got[2].shape == (2, 0, 2, 64) and not any(bool(t.any()) for t in got)
+
+
+# ---- sizes ---------------------------------------------------------------------------------------------------------------------
+
+def test_norm_of_more_rows_than_one_row_of_the_grid_holds(A):
+    """2^26 tokens are 2^32 threads."""
+    N = (1 << 26) + 5
+    q = torch.zeros(1, N, 1, 2, dtype=torch.bfloat16, device="cuda")
+    g = gen(17)
+    for at in (0, (1 << 24) - 3, N - 300):                    # the first, where a row of the grid ends, the last
+        q[:, at:at + 300] = randn(g, 1, 300, 1, 2, dtype=torch.bfloat16)
+    f, pos = A.rope_frequencies(2, device="cuda"), torch.arange(N, device="cuda")
+    y, z = A.qk_norm_rope(q, q, None, None, pos, f)
+    for at in (0, (1 << 24) - 3, N - 300):
+        part = q[:, at:at + 300].contiguous()
+        assert torch.equal(y[:, at:at + 300], A.qk_norm_rope(part, part, None, None, pos[at:at + 300], f)[0])
+    assert torch.equal(y, z)

@@ -223,3 +223,18 @@ def test_strides_of_dimensions_of_one_do_not_matter():
             refused(lib.adk_attention(C.byref(att_args(**docs, **kw)), None, 0, None), "workspace")
         refused(lib.adk_attention_backward(C.byref(att_args(**docs, **kw)), None, 0, None), "workspace")
         refused(lib.adk_attention_backward(C.byref(att_args(**docs, **dict(kw, Nq=2, B=2, Hq=2, Hk=2, Nk=2, k=P, v=P))), None, 0, None), "stride")
+
+
+def test_launches_of_more_threads_than_there_can_be_are_refused():
+    """2^32 threads are the end; what stays below reaches the next check."""
+    lib = _lib.load()
+    docs = dict(documents=P, documents_stride=40)
+    for kw in (dict(B=65535, Hq=512, Hk=512, Nq=1), dict(B=65535, Hq=512, Hk=1, Nq=64), dict(B=65535, Hq=32, Hk=8, Nq=5000)):
+        refused(lib.adk_attention(C.byref(att_args(**kw, **docs)), None, 0, None), "grid")
+    for kw in (dict(B=65535, Hq=256, Hk=128, Nq=1), dict(B=65535, Hq=32, Hk=8, Nq=1), dict(B=1, Hq=8, Hk=8, Nq=1 << 20)):
+        refused(lib.adk_attention(C.byref(att_args(**kw, **docs)), None, 0, None), "workspace")
+    for kw in (dict(B=65535, Hq=256, Hk=128, Nq=1), dict(B=65535, Hq=8, Hk=8, Nk=5000)):
+        refused(lib.adk_attention_backward(C.byref(att_args(**kw, **docs)), None, 0, None), "grid")
+    # few rows over a very long cache: the partial sums stay below 1.2 GB whatever its length
+    for Nk in (1 << 20, 1 << 24, 1 << 28):
+        assert 0 < lib.adk_attention_workspace(C.byref(att_args(B=1, Hq=8, Hk=8, Nq=2040, Nk=Nk, D=128)), 0) < 1.2e9
