@@ -245,3 +245,36 @@ def test_norm_of_more_rows_than_one_row_of_the_grid_holds(A):
         part = q[:, at:at + 300].contiguous()
         assert torch.equal(y[:, at:at + 300], A.qk_norm_rope(part, part, None, None, pos[at:at + 300], f)[0])
     assert torch.equal(y, z)
+
+
+# ---- a scale of one's own ------------------------------------------------------------------------------------------------------
+
+
+def test_gradients_with_offsets_past_2_to_the_31st(A):
+    """Rows, and keys, whose elements are numbered past 2^31: only the last of them have values; every other gradient is zero."""
+    D, tail, few = 64, 200, 70
+    long = (1 << 25) + 37                                     # 2^31 elements of 64
+    g = gen(18)
+
+    def behind(t):
+        wide = torch.zeros(1, long, 1, D, dtype=torch.bfloat16, device="cuda")
+        wide[:, long - tail:] = t
+        return wide
+
+    a, b, c = (randn(g, 1, tail, 1, D, dtype=torch.bfloat16) for _ in range(3))
+    x, y, z = (randn(g, 1, few, 1, D, dtype=torch.bfloat16) for _ in range(3))
+    # many rows, few keys; dO of the rows without values is zero, so they add nothing to dK and dV
+    want = O.attention(a, x, y, grad=b)
+    o, dq, dk, dv = graded(A, behind(a), x, y, behind(b))
+    for n, got in (("o", o[:, long - tail:]), ("dq", dq[:, long - tail:]), ("dk", dk), ("dv", dv)):
+        within(n, got, want[n])
+    assert not bool(dq[:, :long - tail].any())
+    del o, dq, dk, dv
+    # few rows, many keys: a document holds the last of them
+    docs = torch.full((1, long), -1, dtype=torch.int32, device="cuda")
+    docs[:, long - tail:] = 1
+    want = O.attention(x, a, b, grad=z)
+    o, dq, dk, dv = graded(A, x, behind(a), behind(b), z, documents=docs)
+    for n, got in (("o", o), ("dq", dq), ("dk", dk[:, long - tail:]), ("dv", dv[:, long - tail:])):
+        within(n, got, want[n])
+    assert not bool(dk[:, :long - tail].any()) and not bool(dv[:, :long - tail].any())
