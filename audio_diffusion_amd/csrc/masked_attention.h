@@ -367,8 +367,10 @@ __device__ __forceinline__ AtWalk<NW> at_walk(const AttArgs& a, const int* all_r
 // ---- which forward kernel --------------------------------------------------------------------------------------------------
 // The step kernel splits keys over waves and blocks, the other one only query rows.  It takes over where most of a block's rows would be missing
 // (128 rows over 4096 keys, 32 heads of 64: 22 us, otherwise 58), and where those rows alone give too few blocks for 256 CUs.  bf16, step kernel /
-// the other: D = 128, 64 blocks (8 heads, 2048 rows) 46 / 56 us, 128 blocks (4096 rows) 152 / 104; D = 64, 128 blocks (2048 rows) 24 / 32 us, 256 blocks
-// (4096 rows) 83 / 64.
+// the other, 8 heads, as many keys as rows: D = 32, 128 blocks 17.9 / 29.7 us, 248 blocks 41.9 / 51.8; D = 64, 128 blocks 20.7 / 34.4, 192 blocks
+// 47.6 / 48.7, 248 blocks 61.7 / 60.6; D = 128, 64 blocks 44.8 / 56.4, 80 blocks 78.3 / 69.2, 128 blocks 149 / 105.  With 32 heads, hence a quarter of the
+// rows, the blocks at which they meet are fewer (D = 64, 128 blocks 11.8 / 12.9, 192 blocks 25.9 / 16.8; D = 128, 64 blocks 31 / 23): the count of blocks
+// is not all of it (profiles/token_ops/forward_kernels.txt).
 // Its own blocks are split over the keys to fill the card once, at least 512 keys each (below that the joining costs more than it gains:
 // 4096 keys, 8 key heads of 128: 13.8 us, split to 256 keys 15.6) and, so that caches of unequal fill come out even, at most about 4096 (8 caches of 32 to
 // 64 Ki keys: 304 us, four splits of each 323); 2^16 blocks are even enough for any cache, and bound the partial sums.
