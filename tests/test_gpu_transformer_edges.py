@@ -278,3 +278,46 @@ def test_gradients_with_offsets_past_2_to_the_31st(A):
     for n, got in (("o", o), ("dq", dq), ("dk", dk[:, long - tail:]), ("dv", dv[:, long - tail:])):
         within(n, got, want[n])
     assert not bool(dk[:, :long - tail].any()) and not bool(dv[:, :long - tail].any())
+
+
+@pytest.mark.parametrize("D", [32, 64, 128])
+def test_f16_quiet_gradients_beside_infinite_ones_of_padding(A, D):
+    """Infinities and NaN in rows that see nothing take no part in the scale of the others' gradients (2^-8)."""
+    N = 700
+    q, k, v, do, _ = make((2, N, N, 4, 2, D, {}), torch.float16, seed=19)
+    docs = (torch.arange(N, device="cuda") * 7 // N).int().repeat(2, 1)
+    docs[:, 5::9] = -1                                       # padding in every tile
+    rows, do = docs < 0, do * 2.0 ** -8
+    want = O.attention(q, k, v, grad=do, documents=docs, causal=True)
+    g = gen(20)
+    got = graded(A, poison(q, rows, g), poison(k, rows, g), poison(v, rows, g), poison(do, rows, g), documents=docs, causal=True)
+    for n, x in zip(("o", "dq", "dk", "dv"), got):
+        within(n, x[~rows], tuple(t[~rows] for t in want[n]))
+        assert bool((x[rows] == 0).all()), n
+
+
+@pytest.mark.parametrize("softcap", [None, 30.0, 1e4])
+def test_graph_capture_of_f16_gradients(A, softcap):
+    """Forward and backward with all of f16's scratch captured; every replay against the eager result."""
+    g = gen(22)
+    x = [randn(g, 2, 300, 4, 64, dtype=torch.float16) for _ in range(4)]
+    docs = torch.cumsum(torch.rand(2, 300, generator=g, device="cuda") < 0.02, 1).int()
+
+    def step():
+        return graded(A, *x, documents=docs, causal=True, softcap=softcap)
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+    torch.cuda.current_stream().wait_stream(s)
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        out = step()
+    for turn in range(4):
+        for n, t in enumerate(x):
+            t.copy_(randn(g, *t.shape, dtype=t.dtype, scale=4.0 ** (turn - 2) if n == 3 else 1.0))
+        gr.replay()
+        eager = step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, eager)), turn
