@@ -87,7 +87,7 @@ class AttentionArgs(C.Structure):
         i64 documents_stride
         ptr o lse o_grad
         i64 og_stride_b og_stride_n og_stride_h
-        ptr q_grad k_grad v_grad""")
+        ptr q_grad k_grad v_grad o_low""")
 
 
 def packer(mirror):

@@ -599,7 +599,7 @@ int adk_qk_norm_rope_backward(const adk_qk_norm_rope_args* a, void* ws, int64_t 
     return rc ? fail(rc, "qk_norm_rope_backward: launch failed: %s", hipGetErrorString(hipGetLastError())) : ADK_OK;
 }
 
-static int check_att(const AttArgs* a, bool grad, const char* what)
+static int check_att(const adk_attention_args* a, bool grad, const char* what)
 {
     REQUIRE(a, "%s: null arguments", what);
     REQUIRE(a->dtype == ADK_BF16 || a->dtype == ADK_F16, "%s: dtype %d unsupported (bf16 or f16)", what, a->dtype);
@@ -608,11 +608,11 @@ static int check_att(const AttArgs* a, bool grad, const char* what)
     REQUIRE(a->B >= 0 && a->Nq >= 0 && a->Nk >= 0 && a->Nq <= (1 << 28) && a->Nk <= (1 << 28), "%s: B=%d Nq=%d Nk=%d (lengths up to 2^28)",
             what, a->B, a->Nq, a->Nk);
     REQUIRE(a->B <= 65535 && (long long)a->B * a->Hq * ((a->Nq + 31LL) / 32) < (1LL << 30) && (long long)a->B * a->Hk * ((a->Nk + 31LL) / 32) < (1LL << 30)
-            && (long long)a->Nq * (a->Hq / a->Hk) < (1LL << 30) && att_grids_fit(*a, grad), "%s: B=%d x heads %d / %d x rows %d / %d exceed the grid", what,
+            && (long long)a->Nq * (a->Hq / a->Hk) < (1LL << 30) && att_grids_fit(att_args_of(*a), grad), "%s: B=%d x heads %d / %d x rows %d / %d exceed the grid", what,
             a->B, a->Hq, a->Hk, a->Nq, a->Nk);
     REQUIRE(a->scale > 0.f && a->scale <= 3.0e38f, "%s: scale=%g must be positive and finite", what, (double)a->scale);
     REQUIRE(a->softcap >= 0.f && a->softcap <= 3.0e38f, "%s: softcap=%g must be positive and finite, or 0", what, (double)a->softcap);
-    REQUIRE(at_scores_finite(*a), "%s: scale=%g, softcap=%g: 1.45 scale, 2.89 scale / softcap and 2.89 softcap must be within the range of f32", what,
+    REQUIRE(at_scores_finite(att_args_of(*a)), "%s: scale=%g, softcap=%g: 1.45 scale, 2.89 scale / softcap and 2.89 softcap must be within the range of f32", what,
             (double)a->scale, (double)a->softcap);
     REQUIRE(a->causal || !a->prefix, "%s: a prefix mask widens a causal one: set causal", what);
     if (a->B == 0 || a->Nq == 0) return ADK_OK;            // no rows
@@ -623,7 +623,7 @@ static int check_att(const AttArgs* a, bool grad, const char* what)
         return N == 0 || ((a->B == 1 || b % 8 == 0) && (N == 1 || n % 8 == 0) && (H == 1 || h % 8 == 0));
     };
     auto row = [](int N, int64_t s) { return N <= 1 || (s >= 0 && s <= (1 << 24)); };
-    REQUIRE(al(a->q) && al(a->o) && (a->Nk == 0 || (al(a->k) && al(a->v))), "%s: q, k, v and o must be 16-byte aligned", what);
+    REQUIRE(al(a->q) && al(a->o) && al(a->o_low) && (a->Nk == 0 || (al(a->k) && al(a->v))), "%s: q, k, v and o must be 16-byte aligned", what);
     REQUIRE(s8(a->Nq, a->Hq, a->q_stride_b, a->q_stride_n, a->q_stride_h) && s8(a->Nk, a->Hk, a->k_stride_b, a->k_stride_n, a->k_stride_h)
             && s8(a->Nk, a->Hk, a->v_stride_b, a->v_stride_n, a->v_stride_h), "%s: strides must be multiples of 8 elements", what);
     REQUIRE(row(a->Nq, a->q_stride_n) && row(a->Nk, a->k_stride_n) && row(a->Nk, a->v_stride_n) && (!grad || row(a->Nq, a->og_stride_n)),
@@ -639,21 +639,23 @@ static int check_att(const AttArgs* a, bool grad, const char* what)
 int64_t adk_attention_workspace(const adk_attention_args* a, int backward)
 {
     if (check_att(a, false, "attention")) return -1;
-    return backward ? att_backward_workspace(*a) : att_forward_workspace(*a);
+    const AttArgs k = att_args_of(*a);
+    return backward ? att_backward_workspace(k) : att_forward_workspace(k);
 }
 
-static int run_att(const AttArgs* a, void* ws, int64_t ws_bytes, void* stream, bool grad, const char* what)
+static int run_att(const adk_attention_args* a, void* ws, int64_t ws_bytes, void* stream, bool grad, const char* what)
 {
     const int rc = check_att(a, grad, what);
     if (rc) return rc;
     REQUIRE(!grad || a->B == 0 || a->Nq > 0, "%s: no query rows (the gradients of k and v are zeros)", what);
     if (a->B == 0 || a->Nq == 0) return ADK_OK;
-    const long long need = grad ? att_backward_workspace(*a) : att_forward_workspace(*a);
+    const AttArgs k = att_args_of(*a);
+    const long long need = grad ? att_backward_workspace(k) : att_forward_workspace(k);
     REQUIRE(need == 0 || (ws && ((uintptr_t)ws & 15) == 0 && ws_bytes >= need), "%s: workspace of %lld bytes, needs %lld", what,
             (long long)ws_bytes, need);
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-    const int lr = grad ? (a->dtype == ADK_BF16 ? att_backward_bf16(*a, ws, st) : att_backward_f16(*a, ws, st))
-                        : (a->dtype == ADK_BF16 ? att_forward_bf16(*a, ws, st) : att_forward_f16(*a, ws, st));
+    const int lr = grad ? (a->dtype == ADK_BF16 ? att_backward_bf16(k, a->o_low, ws, st) : att_backward_f16(k, a->o_low, ws, st))
+                        : (a->dtype == ADK_BF16 ? att_forward_bf16(k, a->o_low, ws, st) : att_forward_f16(k, a->o_low, ws, st));
     return lr ? fail(lr, "%s: launch failed: %s", what, hipGetErrorString(hipGetLastError())) : ADK_OK;
 }
 

@@ -6,9 +6,35 @@
 // rounded to 16 bits, are the B operand of the next product as they stand: neither scores nor probabilities touch LDS.
 #pragma once
 #include "adk_common.h"
+#include <stddef.h>
+#include <string.h>
 #include <cmath>
 
-typedef adk_attention_args AttArgs;
+// adk_attention_args as the kernels take it: without its last member, o_low, which only some of them use and get beside it.  (The second backward
+// kernel at D = 64 with bias fills its registers to the last one; 8 bytes more of arguments made hipcc spill in its loop.)
+struct AttArgs {
+    int32_t dtype, B, Nq, Nk, Hq, Hk, D, causal;
+    float scale, softcap;
+    const void *q, *k, *v;
+    int64_t q_stride_b, q_stride_n, q_stride_h, k_stride_b, k_stride_n, k_stride_h, v_stride_b, v_stride_n, v_stride_h;
+    const float* slopes;
+    const int32_t *prefix, *lengths, *starts, *documents;
+    int64_t documents_stride;
+    void* o;
+    float* lse;
+    const void* o_grad;
+    int64_t og_stride_b, og_stride_n, og_stride_h;
+    void *q_grad, *k_grad, *v_grad;
+};
+static_assert(sizeof(AttArgs) == offsetof(adk_attention_args, o_low) && offsetof(AttArgs, v_stride_h) == offsetof(adk_attention_args, v_stride_h)
+              && offsetof(AttArgs, documents) == offsetof(adk_attention_args, documents) && offsetof(AttArgs, lse) == offsetof(adk_attention_args, lse)
+              && offsetof(AttArgs, v_grad) == offsetof(adk_attention_args, v_grad), "the same members in the same places");
+static inline AttArgs att_args_of(const adk_attention_args& a)
+{
+    AttArgs k;
+    memcpy(&k, &a, sizeof k);
+    return k;
+}
 typedef __attribute__((ext_vector_type(4))) short att_s16x4;
 
 constexpr int AT_KT = 64;                    // keys of one LDS tile, and of one entry of the document ranges
@@ -325,6 +351,22 @@ template <typename T> __device__ __forceinline__ void at_pack(const f32x16& p, t
     }
 }
 
+// Four elements of a result row from element `at` on, and, where the call wants it (low), what their rounding lost (nothing where they are not finite)
+template <typename T> __device__ __forceinline__ void at_store_o(void* o, void* low, long long at, float x0, float x1, float x2, float x3)
+{
+    uint2 w;
+    w.x = pack2v(f32x2{x0, x1}, T());
+    w.y = pack2v(f32x2{x2, x3}, T());
+    *reinterpret_cast<uint2*>(reinterpret_cast<T*>(o) + at) = w;
+    if (low) {
+        const f32x2 p = unpack2(w.x, T()), q = unpack2(w.y, T());
+        auto lost = [](float x, float r) { const float l = x - r; return l * 0.f == 0.f ? l : 0.f; };
+        w.x = pack2v(f32x2{lost(x0, p.x), lost(x1, p.y)}, T());
+        w.y = pack2v(f32x2{lost(x2, q.x), lost(x3, q.y)}, T());
+        *reinterpret_cast<uint2*>(reinterpret_cast<T*>(low) + at) = w;
+    }
+}
+
 // ---- the key tiles that a block of query rows walks (forward and dQ) -----------------------------------------------------------
 // First and last tile that any row of the block sees, found by all threads over the ranges of documents; tiles between them
 // that miss the block's documents are stepped over.
@@ -399,10 +441,10 @@ static inline bool att_grids_fit(const AttArgs& a, bool grad)
 }
 
 // ---- launchers (one translation unit per type) -----------------------------------------------------------------------------
-int att_forward_bf16(const AttArgs& a, void* ws, hipStream_t st);
-int att_forward_f16(const AttArgs& a, void* ws, hipStream_t st);
-int att_backward_bf16(const AttArgs& a, void* ws, hipStream_t st);
-int att_backward_f16(const AttArgs& a, void* ws, hipStream_t st);
+int att_forward_bf16(const AttArgs& a, void* o_low, void* ws, hipStream_t st);
+int att_forward_f16(const AttArgs& a, void* o_low, void* ws, hipStream_t st);
+int att_backward_bf16(const AttArgs& a, const void* o_low, void* ws, hipStream_t st);
+int att_backward_f16(const AttArgs& a, const void* o_low, void* ws, hipStream_t st);
 int att_launch_doc_ranges(const AttArgs& a, int* ranges, hipStream_t st);
 static inline int att_key_tiles(const AttArgs& a) { return (a.Nk + AT_KT - 1) / AT_KT; }
 constexpr int AT_DOC_LDS = AT_KT * 4;        // documents of a tile, behind its rows

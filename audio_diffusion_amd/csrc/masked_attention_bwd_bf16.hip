@@ -1,7 +1,7 @@
 // bf16 instantiations of masked_attention_bwd.inc
 #include "masked_attention_bwd.inc"
 
-int att_backward_bf16(const AttArgs& a, void* ws, hipStream_t st) { return att_backward_t<bf16_t>(a, ws, st); }
+int att_backward_bf16(const AttArgs& a, const void* o_low, void* ws, hipStream_t st) { return att_backward_t<bf16_t>(a, o_low, ws, st); }
 
 long long att_backward_workspace(const AttArgs& a)
 {

@@ -1,7 +1,7 @@
 // f16 instantiations of masked_attention_bwd.inc, and the scale of every key's dS
 #include "masked_attention_bwd.inc"
 
-int att_backward_f16(const AttArgs& a, void* ws, hipStream_t st) { return att_backward_t<f16_t>(a, ws, st); }
+int att_backward_f16(const AttArgs& a, const void* o_low, void* ws, hipStream_t st) { return att_backward_t<f16_t>(a, o_low, ws, st); }
 
 // The largest |dO| of the rows, of all heads that share the keys, that see each key.  A wave takes 32 keys (key on the lane, half of a
 // tile's rows on each half of the lanes) and looks at the 64-row tiles, first a tile per lane: those that all its keys see whole give their maximum

@@ -158,6 +158,23 @@ __device__ __forceinline__ void at_exact_dkv(const AttArgs& a, const AtScore& sc
     }
 }
 
+// o, and what its rounding lost: see at_store_o
+template <typename T, int D> __device__ __forceinline__ void at_store_o_row(void* o, void* low, long long at, const float (&x)[2], float f)
+{
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        const int e = lane + 64 * u;
+        if (e >= D) break;
+        const float y = x[u] * f;
+        const T r = (T)y;
+        reinterpret_cast<T*>(o)[at + e] = r;
+        if (low) {
+            const float l = y - (float)r;
+            reinterpret_cast<T*>(low)[at + e] = (T)(l * 0.f == 0.f ? l : 0.f);
+        }
+    }
+}
 template <typename T, int D> __device__ __forceinline__ void at_store_row(T* row, const float (&x)[2], float f)
 {
     const int lane = threadIdx.x & 63;

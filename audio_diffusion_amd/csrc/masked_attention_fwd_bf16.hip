@@ -1,7 +1,7 @@
 // bf16 instantiations of masked_attention_fwd.inc, and the document ranges that every kernel of the family reads
 #include "masked_attention_fwd.inc"
 
-int att_forward_bf16(const AttArgs& a, void* ws, hipStream_t st) { return att_forward_t<bf16_t>(a, ws, st); }
+int att_forward_bf16(const AttArgs& a, void* o_low, void* ws, hipStream_t st) { return att_forward_t<bf16_t>(a, o_low, ws, st); }
 
 // smallest and largest document of every 64 keys (padding counts as -1): a tile whose range misses a block's documents is
 // skipped without being loaded

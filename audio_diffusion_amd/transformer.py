@@ -193,19 +193,19 @@ def qk_norm_rope(q, k, q_weight, k_weight, positions, frequencies, eps=1e-6, int
 
 # ---- attention ------------------------------------------------------------------------------------------------------------
 
-def _att_args(q, k, v, slopes, prefix, documents, lengths, starts, causal, scale, softcap, o, lse, grads=_NO_GRAD):
+def _att_args(q, k, v, slopes, prefix, documents, lengths, starts, causal, scale, softcap, o, lse, o_low, grads=_NO_GRAD):
     """AttentionArgs in the order of its fields; grads: the backward call's."""
     B, Nq, Hq, D = q.shape
     return _pack_att(
         _ATT_TYPES[q.dtype], B, Nq, k.shape[1], Hq, k.shape[2], D, causal, scale, softcap, q.data_ptr(), k.data_ptr(), v.data_ptr(),
         *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], _ptr(slopes), _ptr(prefix), _ptr(lengths), _ptr(starts), _ptr(documents),
-        0 if documents is None else documents.stride(0), o.data_ptr(), _ptr(lse), *grads)
+        0 if documents is None else documents.stride(0), o.data_ptr(), _ptr(lse), *grads, _ptr(o_low))
 
 
-def _att_forward(q, k, v, slopes, prefix, documents, lengths, starts, causal, scale, softcap, lse=None):
+def _att_forward(q, k, v, slopes, prefix, documents, lengths, starts, causal, scale, softcap, lse=None, o_low=None):
     lib = _lib.load()
     o = _like(q)
-    a = _att_args(q, k, v, slopes, prefix, documents, lengths, starts, causal, scale, softcap, o, lse)
+    a = _att_args(q, k, v, slopes, prefix, documents, lengths, starts, causal, scale, softcap, o, lse, o_low)
     _launch("masked_attention", q.device, lib.adk_attention, a, lib.adk_attention_workspace(a, 0))
     return o
 
@@ -214,8 +214,9 @@ class _MaskedAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, slopes, prefix, documents, lengths, starts, causal, scale, softcap):
         lse = torch.empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32, device=q.device)
-        o = _att_forward(q, k, v, slopes, prefix, documents, lengths, starts, causal, scale, softcap, lse)
-        ctx.save_for_backward(q, k, v, slopes, prefix, documents, lengths, starts, o, lse)
+        o_low = _like(q)                   # o in 16 bits more, for the gradient's row sums
+        o = _att_forward(q, k, v, slopes, prefix, documents, lengths, starts, causal, scale, softcap, lse, o_low)
+        ctx.save_for_backward(q, k, v, slopes, prefix, documents, lengths, starts, o, lse, o_low)
         ctx.how = (causal, scale, softcap)
         return o
 
@@ -223,13 +224,13 @@ class _MaskedAttention(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, go):
         _no_recording("masked_attention backward", go)
-        q, k, v, slopes, prefix, documents, lengths, starts, o, lse = ctx.saved_tensors
+        q, k, v, slopes, prefix, documents, lengths, starts, o, lse, o_low = ctx.saved_tensors
         dq, dk, dv = _like(q), _like(k), _like(v)
         if q.numel() == 0:
             dk.zero_(), dv.zero_()
         else:
             go = _rows16(go)
-            a = _att_args(q, k, v, slopes, prefix, documents, lengths, starts, *ctx.how, o, lse,
+            a = _att_args(q, k, v, slopes, prefix, documents, lengths, starts, *ctx.how, o, lse, o_low,
                           (go.data_ptr(), *go.stride()[:3], dq.data_ptr(), dk.data_ptr(), dv.data_ptr()))
             lib = _lib.load()
             _launch("masked_attention backward", q.device, lib.adk_attention_backward, a, lib.adk_attention_workspace(a, 1))

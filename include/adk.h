@@ -361,6 +361,9 @@ typedef struct adk_attention_args {
     const void *o_grad;                  /* gradient of o, 16-byte aligned, strides multiples of 8 elements                */
     int64_t og_stride_b, og_stride_n, og_stride_h;
     void *q_grad, *k_grad, *v_grad;      /* [B, Nq, Hq, D], [B, Nk, Hk, D] twice                                           */
+    /* both */
+    void *o_low;                         /* like o, or NULL: what o lost to its rounding (o + o_low is the sum); forward: written, backward: the
+                                            forward's.  Without it delta is taken from the rounded o                        */
 } adk_attention_args;
 
 int adk_sizeof_attention(void);

@@ -321,3 +321,26 @@ def test_graph_capture_of_f16_gradients(A, softcap):
         eager = step()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, eager)), turn
+
+
+# ---- precision of the gradients --------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("case", [(1, 300, 900, 4, 2, 64), (6, 300, 900, 16, 4, 128), (1, 8, 2500, 2, 1, 32)], ids=lambda c: "-".join(map(str, c)))
+def test_gradients_of_scores_of_nearly_equal_values(A, case, dt):
+    """v is one row for all keys and a 2^-6 of noise, so that dP - delta is a small difference of large numbers.  Rounding o alone would
+    put delta off by a third of half a step of the common row, 0.3 u 2^6 of the difference: 4 % in bf16, 0.5 % in f16.  What remains: the rounding of
+    the probabilities in the forward, which the n keys average to 0.6 u 2^6 / sqrt(n) (0.25 %, 0.03 %), of dS and of the result (0.6 u each).
+    Four times that is allowed, of the norm."""
+    B, Nq, Nk, Hq, Hk, D = case
+    q, k, v, do, _ = make(case + ({},), DT[dt], seed=23, scale=0.5)
+    g = gen(24)
+    v = (randn(g, B, 1, Hk, D) + 2.0 ** -6 * v.float()).to(DT[dt])
+    want = O.attention(q, k, v, grad=do)
+    got = graded(A, q, k, v, do)
+    u = torch.finfo(DT[dt]).eps / 2
+    bound = 4 * (0.6 * u * 64 / Nk ** 0.5 + 2 * 0.6 * u)
+    for n, x in zip(("dq", "dk"), got[1:3]):
+        value = want[n][0]
+        off = float((x.double() - value).norm() / value.norm())
+        assert off <= bound, (n, off, bound)
