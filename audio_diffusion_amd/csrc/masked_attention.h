@@ -415,7 +415,7 @@ __device__ __forceinline__ AtWalk<NW> at_walk(const AttArgs& a, const int* all_r
 // is not all of it (profiles/token_ops/forward_kernels.txt).
 // Its own blocks are split over the keys to fill the card once, at least 512 keys each (below that the joining costs more than it gains:
 // 4096 keys, 8 key heads of 128: 13.8 us, split to 256 keys 15.6) and, so that caches of unequal fill come out even, at most about 4096 (8 caches of 32 to
-// 64 Ki keys: 304 us, four splits of each 323); 2^16 blocks are even enough for any cache, and bound the partial sums.
+// 64 Ki keys: 289 us, four splits of each 316); 2^16 blocks are even enough for any cache, and bound the partial sums.
 struct AtStepPlan { bool use; int nsplit; };
 static inline AtStepPlan at_step_plan(const AttArgs& a)
 {

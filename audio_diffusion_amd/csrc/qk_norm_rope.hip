@@ -5,8 +5,8 @@
 //   pairs (p, p + R/2), or (2p, 2p + 1) interleaved, over the first R elements; elements R.. are normed only.
 // Gradient: g = the gradient of y turned back by the angle;  dw = sum_rows g n;  h = g w;  dx = r (h - n mean_d(h n)).
 //
-// Measured, bf16: 4 x 8191 tokens, 32 + 8 heads of 128: 134 us forwards, 212 us gradients (5.0 and 4.7 TB/s; a copy of 2 GiB runs at 4.9
-// here); one token of each of 32 sequences: 5.9 us.
+// Measured, bf16, the kernels alone: 4 x 8191 tokens, 32 + 8 heads of 128: 127 to 138 us forwards, 215 to 229 us gradients (5.3 to 4.9 and 4.7 to 4.4 TB/s;
+// a copy of 2 GiB runs at 4.9 here); one token of each of 32 sequences: 5.7 us.
 // Bound by HBM: every element is read once and written once (gradient: two reads, one write), with 16-byte accesses.
 // A wave takes one TOKEN and walks its heads: the angles of a token are the same for all heads, so each lane computes one of
 // them (in 64 bits up to the fraction of a turn: exact for any position a 64-bit product holds), the wave shares them through
